@@ -652,6 +652,55 @@ int sm3_gfl_loss_bwd(const float* cls, const float* bbox, const float* anchors, 
                      const int64_t* gt_labels, const int* gt_off, const uint8_t* valid, float pos_weight, float beta,
                      const float* coef, float* dcls, float* dbbox, sm3_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------------------------
+ * Products grouped by expert in 16 bits, with their gradients, and microscaled 4-bit (MXFP4) quantisation and products: the
+ * expert loop of MoE_layer.forward (convnext_moe.py:243-245) and FFN.forward (:397-405) for bf16 / fp16 training and 4-bit
+ * inference.  Types of tensors: */
+#define SM3_DT_F32 0
+#define SM3_DT_F16 1
+#define SM3_DT_BF16 2
+/* MXFP4 rows: blocks of 32 consecutive elements of a row share the scale 2^(byte - 127); elements are e2m1 (0 .5 1 1.5 2 3 4 6
+ * and sign).  k elements are padded with zeros to kp = k rounded up to a multiple of 128.  codes (rows, kp / 2): element 2 i in
+ * the low, 2 i + 1 in the high nibble of byte i; scales (rows, kp / 32).
+ * quantize: byte = max(floor(log2 max|x|) - 2 + 127, 0); elements round to nearest, ties to the even code, beyond 6 to 6; a block
+ * that holds an infinity or a NaN gets byte 255 (the whole block is NaN).  x: `rows` rows of k elements, ld elements apart.
+ * dequantize: y (rows, k) contiguous, rounded to nearest even. */
+int sm3_mx4_quantize(const void* x, int type, long rows, int k, long ld, uint8_t* codes, uint8_t* scales,
+                     sm3_stream_t stream);
+int sm3_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, long rows, int k, void* y, int type,
+                       sm3_stream_t stream);
+/* Grouped products.  `offsets`: DEVICE int32[num_groups + 1], rows [offsets[g], offsets[g+1]) of p belong to expert g (clamped
+ * to [0, rows] and made monotone by the kernels); NULL: num_groups == 1, every row.  Rows of no expert get zeros.
+ *   mode SM3_GEMM_NT: out (rows, cols) = act(p (rows, red) . q[g] (cols, red)^T + bias[g])
+ *   mode SM3_GEMM_NN: out (rows, cols) = p (rows, red) . q[g] (red, cols)
+ *   mode SM3_GEMM_TN: out[g] (rows_out, cols) = p (rows of g, rows_out)^T . q (rows of g, cols); bias_grad[g] (rows_out) = column
+ *                     sums of p over the rows of g (may be NULL).  Experts without rows get zeros.
+ * 16-bit: p, q of type `type` (F16 | BF16), 16-byte aligned, ldp / ldq elements between rows (multiples of 8; elements behind
+ * the row's end up to the next multiple of 8 are read and must be ZERO along the reduction); NT / NN weights of expert g start
+ * at q + g * cols * ldq (NN: g * red * ldq).  out contiguous, of type `out_type` (16-bit: equal to `type`).
+ * MX4: NT only; p / q = codes, p_scales / q_scales, red = k (padded rows as above), ldp / ldq ignored.
+ * act: 0 none, 1 GELU (erf).  bias (num_groups, cols) / bias_grad (num_groups, rows_out) of type bias_type. */
+typedef struct sm3_expert_desc {
+  int32_t mode, type, out_type, bias_type, act, num_groups;
+  int32_t red, cols, rows_out, reserved;
+  int64_t rows, ldp, ldq;
+  const void* p;
+  const void* q;
+  const uint8_t* p_scales;
+  const uint8_t* q_scales;
+  const int32_t* offsets;
+  const void* bias;
+  void* bias_grad;
+  void* out;
+} sm3_expert_desc;
+size_t sm3_expert_gemm_h16_workspace_bytes(const sm3_expert_desc* desc);
+int sm3_expert_gemm_h16(const sm3_expert_desc* desc, void* workspace, size_t workspace_bytes, sm3_stream_t stream);
+size_t sm3_mx4_gemm_workspace_bytes(const sm3_expert_desc* desc);
+int sm3_mx4_gemm(const sm3_expert_desc* desc, void* workspace, size_t workspace_bytes, sm3_stream_t stream);
+/* dst (rows, kp) = src (rows, k; ld elements apart) of a 16-bit type, columns k .. kp - 1 zero: rows that are not 16-byte
+ * aligned or not a multiple of 8 long, made readable for sm3_expert_gemm_h16.  kp % 8 == 0, kp >= k, dst 16-byte aligned. */
+int sm3_pad_rows_h16(const void* src, long rows, int k, long ld, void* dst, int kp, sm3_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -26,8 +26,17 @@ class GemmDesc(ctypes.Structure):
     ]
 
 
+class ExpertDesc(ctypes.Structure):
+    """mirror of `sm3_expert_desc` (include/sm3det_hip.h)"""
+    _fields_ = [(n, ctypes.c_int32) for n in ('mode', 'type', 'out_type', 'bias_type', 'act', 'num_groups', 'red', 'cols',
+                                              'rows_out', 'reserved')] + \
+               [(n, ctypes.c_int64) for n in ('rows', 'ldp', 'ldq')] + \
+               [(n, P) for n in ('p', 'q', 'p_scales', 'q_scales', 'offsets', 'bias', 'bias_grad', 'out')]
+
+
 def signatures():
     D = ctypes.POINTER(GemmDesc)
+    XD = ctypes.POINTER(ExpertDesc)
     LL = ctypes.c_long
     return {
         'sm3_gemm_f32_counter_slots': (I, []),
@@ -88,6 +97,13 @@ def signatures():
         'sm3_deform_col2im_nhwc': (I, [P, P, P] + [I] * 13 + [LL, P]),
         'sm3_deform_bwd_input_fused': (I, [P, P, P, P, P] + [I] * 13 + [LL, P]),
         'sm3_deform_col2im_coord': (I, [P, P, P, P] + [I] * 13 + [LL, P]),
+        'sm3_mx4_quantize': (I, [P, I, LL, I, LL, P, P, P]),
+        'sm3_mx4_dequantize': (I, [P, P, LL, I, P, I, P]),
+        'sm3_expert_gemm_h16_workspace_bytes': (S, [XD]),
+        'sm3_expert_gemm_h16': (I, [XD, P, S, P]),
+        'sm3_mx4_gemm_workspace_bytes': (S, [XD]),
+        'sm3_mx4_gemm': (I, [XD, P, S, P]),
+        'sm3_pad_rows_h16': (I, [P, LL, I, LL, P, I, P]),
     }
 
 

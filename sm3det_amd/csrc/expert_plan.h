@@ -1,0 +1,239 @@
+// expert_plan.h -- host side of the grouped products: checks, launch shapes, workspaces, the joins of split reductions.
+#pragma once
+#include "expert_tile.h"
+
+namespace sm3x {
+
+// rows a grid has to provide for: every expert may end in a part-filled tile, and so may the rows before the first and behind
+// the last expert
+inline long row_tiles(long S, int G, bool grouped, long bm) {
+  if (!grouped) return (S + bm - 1) / bm;
+  return S / bm + (S < G ? S : G) + 2;
+}
+
+struct Plan {
+  int bm, bn;          // tile
+  long mtiles;
+  int ntiles, splits;  // NT / NN: slices of the reduction
+  long unit_rows, units;  // TN: reduction rows per work unit
+  size_t part_bytes, bsum_bytes;
+};
+
+inline int check_desc(const sm3_expert_desc* d, bool mx4) {
+  if (!d || d->num_groups < 1 || d->rows < 0 || d->rows > 0x7fffff00L || d->red < 1 || d->cols < 1) return SM3_ERR_INVALID_ARG;
+  if (d->mode < SM3_GEMM_NT || d->mode > SM3_GEMM_TN || (mx4 && d->mode != SM3_GEMM_NT)) return SM3_ERR_INVALID_ARG;
+  if (!d->offsets && d->num_groups != 1) return SM3_ERR_INVALID_ARG;
+  if (d->act < 0 || d->act > 1 || d->bias_type < 0 || d->bias_type > SM3_DT_BF16) return SM3_ERR_INVALID_ARG;
+  if (d->out_type < 0 || d->out_type > SM3_DT_BF16) return SM3_ERR_INVALID_ARG;
+  if (d->mode == SM3_GEMM_TN ? d->rows_out < 1 || d->bias || d->act : d->bias_grad != nullptr) return SM3_ERR_INVALID_ARG;
+  const bool reads = d->rows > 0;  // (a weight gradient over no rows writes zeros)
+  if (!d->out || (reads && (!d->p || !d->q))) return SM3_ERR_INVALID_ARG;
+  if ((uintptr_t)d->p % 16 || (uintptr_t)d->q % 16) return SM3_ERR_INVALID_ARG;
+  // 32-bit offsets inside a tile: 256 rows of either operand
+  const long most = 1L << 22;
+  if (mx4) {
+    if (!d->p_scales || !d->q_scales || (uintptr_t)d->p_scales % 4 || (uintptr_t)d->q_scales % 4) return SM3_ERR_INVALID_ARG;
+    if (d->red > most) return SM3_ERR_UNSUPPORTED;
+  } else {
+    if (d->type != SM3_DT_F16 && d->type != SM3_DT_BF16) return SM3_ERR_INVALID_ARG;
+    if (d->out_type != d->type) return SM3_ERR_INVALID_ARG;
+    const long prow = d->mode == SM3_GEMM_TN ? d->rows_out : d->red, qrow = d->mode == SM3_GEMM_NT ? d->red : d->cols;
+    if (d->ldp % 8 || d->ldq % 8 || d->ldp < (prow + 7) / 8 * 8 || d->ldq < (qrow + 7) / 8 * 8) return SM3_ERR_INVALID_ARG;
+    if (d->ldp > most || d->ldq > most) return SM3_ERR_UNSUPPORTED;
+  }
+  return SM3_OK;
+}
+
+inline Plan make_plan(const sm3_expert_desc* d, bool mx4) {
+  Plan p{};
+  const bool grouped = d->offsets != nullptr;
+  if (d->mode == SM3_GEMM_TN) {
+    p.bm = p.bn = 128;
+    p.ntiles = (d->cols + p.bn - 1) / p.bn;
+    const long mt = (d->rows_out + p.bm - 1) / p.bm, tiles = mt * p.ntiles;
+    // too few tiles to fill the chip: the reduction is cut into units whose fp32 partials a second launch adds in order
+    p.unit_rows = d->rows > 0 ? d->rows : 1;
+    p.units = d->num_groups;
+    if (tiles * d->num_groups < 2 * kNumCU) {
+      long want = (3L * kNumCU + tiles - 1) / tiles;
+      long r = (d->rows + want - 1) / want;
+      r = (r + kStepRed - 1) / kStepRed * kStepRed;
+      if (r < 4 * kStepRed) r = 4 * kStepRed;
+      if (r < d->rows) {
+        p.unit_rows = r;
+        p.units = d->rows / r + d->num_groups;
+        p.part_bytes = align_up((size_t)p.units * d->rows_out * d->cols * 4, 256);
+        if (d->bias_grad) p.bsum_bytes = align_up((size_t)p.units * d->rows_out * 4, 256);
+      }
+    }
+    if (!p.part_bytes && d->bias_grad) p.bsum_bytes = align_up((size_t)p.units * d->rows_out * 4, 256);
+    p.mtiles = p.units * mt;
+    p.splits = 1;
+    return p;
+  }
+  const long per_expert = d->rows / (d->num_groups < d->rows ? d->num_groups : d->rows > 0 ? d->rows : 1);
+  p.bm = per_expert <= 48 ? 32 : 128;
+  p.bn = 128;
+  p.ntiles = (d->cols + p.bn - 1) / p.bn;
+  p.mtiles = row_tiles(d->rows, d->num_groups, grouped, p.bm);
+  p.splits = 1;
+  const long steps = ((mx4 ? (d->red + 127) / 128 * 64 : d->red * 2L) + kStepBytes - 1) / kStepBytes;
+  const long tiles = p.mtiles * p.ntiles;
+  if (tiles < kNumCU && steps >= 8) {
+    long s = (2L * kNumCU + tiles - 1) / tiles;
+    if (s > steps / 4) s = steps / 4;
+    if (s > 16) s = 16;
+    if (s > 1) {
+      p.splits = (int)s;
+      p.part_bytes = align_up((size_t)s * d->rows * d->cols * 4, 256);
+    }
+  }
+  return p;
+}
+
+// ---- joins --------------------------------------------------------------------------------------------------------
+// out[s][n] = act(sum over slices + bias of the row's expert); one row per blockIdx.y
+static __global__ void __launch_bounds__(256) join_rows_kernel(const Params P) {
+  const long n = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
+  for (long s = blockIdx.y; s < P.S; s += gridDim.y) {
+    int g = P.offsets ? -1 : 0;
+    if (P.offsets) {  // first expert whose end lies behind the row
+      const int lane = threadIdx.x & 63;
+      for (int b = 0; b < P.G && g < 0; b += 64) {
+        const unsigned long long hit = __ballot(b + lane < P.G && P.offsets[b + lane + 1] > s);
+        if (hit) g = b + __ffsll(hit) - 1;
+      }
+      if (s < P.offsets[0]) g = -1;
+    }
+    if (n >= P.cols) continue;
+    const int have = (int)(P.cols - n < 4 ? P.cols - n : 4);
+    v4f v = {0.f, 0.f, 0.f, 0.f};
+    for (int z = 0; z < P.splits; z++)
+      for (int r = 0; r < 4; r++) { if (r < have) v[r] += P.part[((long)z * P.S + s) * P.cols + n + r]; }
+    if (g >= 0) {
+      for (int r = 0; r < 4; r++) {
+        if (P.bias && r < have) v[r] += load_bias(P.bias, P.bias_type, (long)g * P.cols + n + r);
+        if (P.act) v[r] = gelu(v[r]);
+      }
+    }
+    store4(P.out, P.out_type, s * P.cols + n, v, have, P.vec);
+  }
+}
+
+// out[g][i] = sum over the work units of expert g, in their order; `n` values per unit
+static __global__ void __launch_bounds__(256) join_units_kernel(const float* __restrict__ part, const Params P, void* out,
+                                                                int type, long n, int vec) {
+  const int g = blockIdx.y, lane = threadIdx.x & 63;
+  long first = 0;
+  int count = 0;
+  const int S = (int)P.S;
+  if (P.offsets == nullptr) {
+    count = S > 0 ? (int)((S + P.unit_rows - 1) / P.unit_rows) : 1;
+  } else {
+    int carry = P.offsets[0];
+    carry = carry < 0 ? 0 : carry > S ? S : carry;
+    for (int b = 0; b <= g; b += 64) {
+      int end = b + lane < P.G ? P.offsets[b + lane + 1] : 0;
+      end = end < 0 ? 0 : end > S ? S : end;
+      end = end < carry ? carry : end;
+      for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(end, d);
+        if (lane >= d && o > end) end = o;
+      }
+      int start = __shfl_up(end, 1);
+      if (lane == 0) start = carry;
+      int u = b + lane < P.G ? (int)((end - start + P.unit_rows - 1) / P.unit_rows) : 0;
+      if (b + lane < P.G && u == 0) u = 1;
+      int incl = u;
+      for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(incl, d);
+        if (lane >= d) incl += o;
+      }
+      if (g < b + 64) {
+        count = __shfl(u, g - b);
+        first += __shfl(incl, g - b) - count;
+      } else {
+        first += __shfl(incl, 63);
+        carry = __shfl(end, 63);
+      }
+    }
+  }
+  const long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  const int have = (int)(n - i < 4 ? n - i : 4);
+  v4f v = {0.f, 0.f, 0.f, 0.f};
+  for (int u = 0; u < count; u++) {
+    const float* at = part + (first + u) * n + i;
+    if (vec) v += *(const v4f*)at;
+    else
+      for (int r = 0; r < 4; r++) { if (r < have) v[r] += at[r]; }
+  }
+  store4(out, type, (long)g * n + i, v, have, vec);
+}
+
+inline int out_vec(const void* out, int type, long cols) {  // four columns in one store
+  return cols % 4 == 0 && (uintptr_t)out % (type == SM3_DT_F32 ? 16 : 8) == 0;
+}
+
+inline Params params_of(const sm3_expert_desc* d, const Plan& pl, bool mx4, void* ws) {
+  Params P{};
+  P.p = (const char*)d->p;
+  P.q = (const char*)d->q;
+  P.S = d->rows;
+  P.G = d->num_groups;
+  P.offsets = d->offsets;
+  P.out = d->out;
+  P.out_type = d->out_type;
+  P.bias = d->bias;
+  P.bias_type = d->bias_type;
+  P.act = d->act;
+  P.cols = d->cols;
+  P.rows_out = d->rows_out;
+  P.vec = out_vec(d->out, d->out_type, d->cols);
+  if (mx4) {
+    const long kp = (d->red + 127) / 128 * 128;
+    P.ldp = P.ldq = P.red = kp / 2;
+    P.ldps = P.ldqs = kp / 32;
+    P.strideq = d->cols * P.ldq;
+    P.strideqs = d->cols * P.ldqs;
+    P.ps = d->p_scales;
+    P.qs = d->q_scales;
+  } else {
+    P.ldp = d->ldp * 2;
+    P.ldq = d->ldq * 2;
+    P.red = d->red * 2L;
+    P.qred = d->red;
+    P.strideq = (d->mode == SM3_GEMM_NT ? (long)d->cols : (long)d->red) * P.ldq;
+    // 16-byte granules that straddle the end of the reduction hold zeros behind it (the caller's rows are padded)
+    if (d->mode != SM3_GEMM_TN) P.red = (P.red + 15) & ~15L;
+  }
+  P.ntiles = pl.ntiles;
+  P.mtiles = pl.mtiles;
+  P.splits = pl.splits;
+  P.unit_rows = pl.unit_rows;
+  P.part = pl.part_bytes ? (float*)ws : nullptr;
+  P.bsum = pl.bsum_bytes ? (float*)((char*)ws + pl.part_bytes) : nullptr;
+  return P;
+}
+
+inline dim3 grid_of(const Plan& pl) {
+  const long total = pl.mtiles * pl.ntiles, per = (total + kNumXCD - 1) / kNumXCD;
+  return dim3((unsigned)(per * kNumXCD), (unsigned)pl.splits);
+}
+
+inline int finish(const Params& P, const Plan& pl, const sm3_expert_desc* d, hipStream_t st) {
+  if (d->mode == SM3_GEMM_TN) {
+    const long n = (long)P.rows_out * P.cols;
+    if (P.part)
+      join_units_kernel<<<dim3((unsigned)((n + 1023) / 1024), P.G), 256, 0, st>>>(P.part, P, P.out, P.out_type, n,
+                                                                                n % 4 == 0 && out_vec(P.out, P.out_type, n));
+    if (P.bsum)
+      join_units_kernel<<<dim3((unsigned)((P.rows_out + 1023) / 1024), P.G), 256, 0, st>>>(
+          P.bsum, P, d->bias_grad, d->bias_type, P.rows_out, P.rows_out % 4 == 0 && out_vec(d->bias_grad, d->bias_type, P.rows_out));
+  } else if (P.part) {
+    join_rows_kernel<<<dim3((unsigned)((P.cols + 1023) / 1024), (unsigned)(P.S < 32768 ? P.S : 32768)), 256, 0, st>>>(P);
+  }
+  return launch_status();
+}
+
+}  // namespace sm3x

@@ -1,0 +1,29 @@
+// mx4_gemm.hip -- products of microscaled 4-bit rows, dense and grouped by expert: v_mfma_scale_f32_16x16x128_f8f6f4 with both
+// operands e2m1 and the blocks' scale bytes as its scale operands (no dequantised copy exists anywhere).
+#include "expert_plan.h"
+
+using namespace sm3x;
+
+extern "C" {
+
+size_t sm3_mx4_gemm_workspace_bytes(const sm3_expert_desc* d) {
+  if (check_desc(d, true) != SM3_OK) return 0;
+  return make_plan(d, true).part_bytes;
+}
+
+int sm3_mx4_gemm(const sm3_expert_desc* d, void* workspace, size_t workspace_bytes, sm3_stream_t stream) {
+  const int err = check_desc(d, true);
+  if (err != SM3_OK) return err;
+  if (d->rows == 0) return SM3_OK;
+  const Plan pl = make_plan(d, true);
+  if (pl.part_bytes && (!workspace || workspace_bytes < pl.part_bytes || (uintptr_t)workspace % 16)) return SM3_ERR_WORKSPACE;
+  const Params P = params_of(d, pl, true, workspace);
+  hipStream_t st = (hipStream_t)stream;
+  const dim3 grid = grid_of(pl);
+  if (pl.bm == 32) tile_kernel<K_MX4, M_NT, 32, 128, 1, 4><<<grid, 256, 0, st>>>(P);
+  else tile_kernel<K_MX4, M_NT, 128, 128, 2, 2><<<grid, 256, 0, st>>>(P);
+  const int rc = launch_status();
+  return rc != SM3_OK ? rc : finish(P, pl, d, st);
+}
+
+}  // extern "C"

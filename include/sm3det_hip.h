@@ -679,7 +679,7 @@ int sm3_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, long rows, i
  * the row's end up to the next multiple of 8 are read and must be ZERO along the reduction); NT / NN weights of expert g start
  * at q + g * cols * ldq (NN: g * red * ldq).  out contiguous, of type `out_type` (16-bit: equal to `type`).
  * MX4: NT only; p / q = codes, p_scales / q_scales, red = k (padded rows as above), ldp / ldq ignored.
- * act: 0 none, 1 GELU (erf).  bias (num_groups, cols) / bias_grad (num_groups, rows_out) of type bias_type. */
+ * act: 0 none, 1 GELU (erf; MX4 only).  bias (num_groups, cols) / bias_grad (num_groups, rows_out) of type bias_type. */
 typedef struct sm3_expert_desc {
   int32_t mode, type, out_type, bias_type, act, num_groups;
   int32_t red, cols, rows_out, reserved;

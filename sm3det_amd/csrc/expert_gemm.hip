@@ -6,18 +6,17 @@ using namespace sm3x;
 
 namespace {
 
+template <int KIND, int MODE>
+void launch_mode(const Params& P, const Plan& pl, hipStream_t st) {
+  if (MODE != M_TN && pl.bm == 32) tile_kernel<KIND, MODE == M_TN ? M_NT : MODE, 32, 128, 1, 4, 2><<<grid_of(pl, 3), 256, 0, st>>>(P);
+  else tile_kernel<KIND, MODE, 128, 128, 2, 2, 2><<<grid_of(pl, 2), 256, 0, st>>>(P);
+}
+
 template <int KIND>
 int launch(const Params& P, const Plan& pl, int mode, hipStream_t st) {
-  const dim3 grid = grid_of(pl);
-  if (mode == SM3_GEMM_NT) {
-    if (pl.bm == 32) tile_kernel<KIND, M_NT, 32, 128, 1, 4><<<grid, 256, 0, st>>>(P);
-    else tile_kernel<KIND, M_NT, 128, 128, 2, 2><<<grid, 256, 0, st>>>(P);
-  } else if (mode == SM3_GEMM_NN) {
-    if (pl.bm == 32) tile_kernel<KIND, M_NN, 32, 128, 1, 4><<<grid, 256, 0, st>>>(P);
-    else tile_kernel<KIND, M_NN, 128, 128, 2, 2><<<grid, 256, 0, st>>>(P);
-  } else {
-    tile_kernel<KIND, M_TN, 128, 128, 2, 2><<<grid, 256, 0, st>>>(P);
-  }
+  if (mode == SM3_GEMM_NT) launch_mode<KIND, M_NT>(P, pl, st);
+  else if (mode == SM3_GEMM_NN) launch_mode<KIND, M_NN>(P, pl, st);
+  else launch_mode<KIND, M_TN>(P, pl, st);
   return launch_status();
 }
 
@@ -51,6 +50,7 @@ int sm3_expert_gemm_h16(const sm3_expert_desc* d, void* workspace, size_t worksp
   if (d->mode != SM3_GEMM_TN && d->rows == 0) return SM3_OK;
   const Plan pl = make_plan(d, false);
   const size_t need = pl.part_bytes + pl.bsum_bytes;
+  if (!fits(pl)) return SM3_ERR_UNSUPPORTED;
   if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16)) return SM3_ERR_WORKSPACE;
   const Params P = params_of(d, pl, false, workspace);
   hipStream_t st = (hipStream_t)stream;

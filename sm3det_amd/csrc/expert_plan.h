@@ -13,11 +13,14 @@ inline long row_tiles(long S, int G, bool grouped, long bm) {
 
 struct Plan {
   int bm, bn;          // tile
-  long mtiles;
+  long mtiles, per_xcd;  // row tiles; jobs of one XCD
   int ntiles, splits;  // NT / NN: slices of the reduction
   long unit_rows, units;  // TN: reduction rows per work unit
   size_t part_bytes, bsum_bytes;
 };
+
+// jobs are counted in 31 bits
+inline bool fits(const Plan& p) { return (double)p.per_xcd * kNumXCD < 2.0e9 && (double)p.units < 2.0e9; }
 
 inline int check_desc(const sm3_expert_desc* d, bool mx4) {
   if (!d || d->num_groups < 1 || d->rows < 0 || d->rows > 0x7fffff00L || d->red < 1 || d->cols < 1) return SM3_ERR_INVALID_ARG;
@@ -36,7 +39,7 @@ inline int check_desc(const sm3_expert_desc* d, bool mx4) {
     if (d->red > most) return SM3_ERR_UNSUPPORTED;
   } else {
     if (d->type != SM3_DT_F16 && d->type != SM3_DT_BF16) return SM3_ERR_INVALID_ARG;
-    if (d->out_type != d->type) return SM3_ERR_INVALID_ARG;
+    if (d->out_type != d->type || d->act) return SM3_ERR_INVALID_ARG;
     const long prow = d->mode == SM3_GEMM_TN ? d->rows_out : d->red, qrow = d->mode == SM3_GEMM_NT ? d->red : d->cols;
     if (d->ldp % 8 || d->ldq % 8 || d->ldp < (prow + 7) / 8 * 8 || d->ldq < (qrow + 7) / 8 * 8) return SM3_ERR_INVALID_ARG;
     if (d->ldp > most || d->ldq > most) return SM3_ERR_UNSUPPORTED;
@@ -69,6 +72,7 @@ inline Plan make_plan(const sm3_expert_desc* d, bool mx4) {
     if (!p.part_bytes && d->bias_grad) p.bsum_bytes = align_up((size_t)p.units * d->rows_out * 4, 256);
     p.mtiles = p.units * mt;
     p.splits = 1;
+    p.per_xcd = p.units * ((tiles + kNumXCD - 1) / kNumXCD);
     return p;
   }
   const long per_expert = d->rows / (d->num_groups < d->rows ? d->num_groups : d->rows > 0 ? d->rows : 1);
@@ -88,17 +92,17 @@ inline Plan make_plan(const sm3_expert_desc* d, bool mx4) {
       p.part_bytes = align_up((size_t)s * d->rows * d->cols * 4, 256);
     }
   }
+  p.per_xcd = (tiles * p.splits + kNumXCD - 1) / kNumXCD;
   return p;
 }
 
 // ---- joins --------------------------------------------------------------------------------------------------------
-// out[s][n] = act(sum over slices + bias of the row's expert); one row per blockIdx.y
+// out[s][n] = act(sum over slices + bias of the row's expert); eight columns of a row per thread
 static __global__ void __launch_bounds__(256) join_rows_kernel(const Params P) {
-  const long n = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
+  const int n = (blockIdx.x * 256 + threadIdx.x) * 8, lane = threadIdx.x & 63;
   for (long s = blockIdx.y; s < P.S; s += gridDim.y) {
     int g = P.offsets ? -1 : 0;
     if (P.offsets) {  // first expert whose end lies behind the row
-      const int lane = threadIdx.x & 63;
       for (int b = 0; b < P.G && g < 0; b += 64) {
         const unsigned long long hit = __ballot(b + lane < P.G && P.offsets[b + lane + 1] > s);
         if (hit) g = b + __ffsll(hit) - 1;
@@ -106,23 +110,29 @@ static __global__ void __launch_bounds__(256) join_rows_kernel(const Params P) {
       if (s < P.offsets[0]) g = -1;
     }
     if (n >= P.cols) continue;
-    const int have = (int)(P.cols - n < 4 ? P.cols - n : 4);
-    v4f v = {0.f, 0.f, 0.f, 0.f};
-    for (int z = 0; z < P.splits; z++)
-      for (int r = 0; r < 4; r++) { if (r < have) v[r] += P.part[((long)z * P.S + s) * P.cols + n + r]; }
-    if (g >= 0) {
-      for (int r = 0; r < 4; r++) {
-        if (P.bias && r < have) v[r] += load_bias(P.bias, P.bias_type, (long)g * P.cols + n + r);
-        if (P.act) v[r] = gelu(v[r]);
-      }
+    const int have = P.cols - n;
+    float v[8] = {};
+    for (int z = 0; z < P.splits; z++) {
+      const float* at = P.part + ((long)z * P.S + s) * P.cols + n;
+#pragma unroll
+      for (int r = 0; r < 8; r++) v[r] += r < have ? at[r] : 0.f;
     }
-    store4(P.out, P.out_type, s * P.cols + n, v, have, P.vec);
+    if (g >= 0) {
+      if (P.bias) {
+        float b[8];
+        bias8(b, P.bias, P.bias_type, (long)g * P.cols + n, (long)g * P.cols + P.cols - 1);
+#pragma unroll
+        for (int r = 0; r < 8; r++) v[r] += b[r];
+      }
+      if (P.act) gelu8(v);
+    }
+    store8(P.out, P.out_type, s * P.cols + n, v, have, P.cols % (P.out_type == DT_F32 ? 4 : 8) == 0 && (uintptr_t)P.out % 16 == 0);
   }
 }
 
 // out[g][i] = sum over the work units of expert g, in their order; `n` values per unit
 static __global__ void __launch_bounds__(256) join_units_kernel(const float* __restrict__ part, const Params P, void* out,
-                                                                int type, long n, int vec) {
+                                                                int type, long n) {
   const int g = blockIdx.y, lane = threadIdx.x & 63;
   long first = 0;
   int count = 0;
@@ -158,21 +168,26 @@ static __global__ void __launch_bounds__(256) join_units_kernel(const float* __r
       }
     }
   }
-  const long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
+  const long i = ((long)blockIdx.x * 256 + threadIdx.x) * 8;
   if (i >= n) return;
-  const int have = (int)(n - i < 4 ? n - i : 4);
-  v4f v = {0.f, 0.f, 0.f, 0.f};
+  const int have = (int)(n - i < 8 ? n - i : 8);
+  float v[8] = {};
+  const bool whole = n % 8 == 0;
   for (int u = 0; u < count; u++) {
     const float* at = part + (first + u) * n + i;
-    if (vec) v += *(const v4f*)at;
-    else
-      for (int r = 0; r < 4; r++) { if (r < have) v[r] += at[r]; }
+    if (whole) {
+      const v4f lo = *(const v4f*)at, hi = *(const v4f*)(at + 4);
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        v[r] += lo[r];
+        v[r + 4] += hi[r];
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < 8; r++) v[r] += r < have ? at[r] : 0.f;
+    }
   }
-  store4(out, type, (long)g * n + i, v, have, vec);
-}
-
-inline int out_vec(const void* out, int type, long cols) {  // four columns in one store
-  return cols % 4 == 0 && (uintptr_t)out % (type == SM3_DT_F32 ? 16 : 8) == 0;
+  store8(out, type, (long)g * n + i, v, have, whole && (uintptr_t)out % 16 == 0);
 }
 
 inline Params params_of(const sm3_expert_desc* d, const Plan& pl, bool mx4, void* ws) {
@@ -189,7 +204,6 @@ inline Params params_of(const sm3_expert_desc* d, const Plan& pl, bool mx4, void
   P.act = d->act;
   P.cols = d->cols;
   P.rows_out = d->rows_out;
-  P.vec = out_vec(d->out, d->out_type, d->cols);
   if (mx4) {
     const long kp = (d->red + 127) / 128 * 128;
     P.ldp = P.ldq = P.red = kp / 2;
@@ -208,30 +222,33 @@ inline Params params_of(const sm3_expert_desc* d, const Plan& pl, bool mx4, void
     if (d->mode != SM3_GEMM_TN) P.red = (P.red + 15) & ~15L;
   }
   P.ntiles = pl.ntiles;
-  P.mtiles = pl.mtiles;
   P.splits = pl.splits;
   P.unit_rows = pl.unit_rows;
   P.part = pl.part_bytes ? (float*)ws : nullptr;
+  const long bes = d->bias_type == SM3_DT_F32 ? 4 : 2;
+  P.bias_lds = d->bias && (uintptr_t)d->bias % 4 == 0 && d->cols * bes % 4 == 0;
+  P.wide = P.part ? d->cols % 4 == 0 : d->cols % (d->out_type == SM3_DT_F32 ? 4 : 8) == 0 && (uintptr_t)d->out % 16 == 0;
   P.bsum = pl.bsum_bytes ? (float*)((char*)ws + pl.part_bytes) : nullptr;
   return P;
 }
 
-inline dim3 grid_of(const Plan& pl) {
-  const long total = pl.mtiles * pl.ntiles, per = (total + kNumXCD - 1) / kNumXCD;
-  return dim3((unsigned)(per * kNumXCD), (unsigned)pl.splits);
+// as many workgroups as are resident at once (a multiple of the XCDs), each with its share of the jobs -- at most kMaxJobs of them
+inline dim3 grid_of(const Plan& pl, int per_cu) {
+  const long most = (long)kNumCU / kNumXCD * per_cu, least = (pl.per_xcd + kMaxJobs - 1) / kMaxJobs;
+  const long each = pl.per_xcd < most ? pl.per_xcd : most > least ? most : least;
+  return dim3((unsigned)(each * kNumXCD));
 }
 
 inline int finish(const Params& P, const Plan& pl, const sm3_expert_desc* d, hipStream_t st) {
   if (d->mode == SM3_GEMM_TN) {
     const long n = (long)P.rows_out * P.cols;
     if (P.part)
-      join_units_kernel<<<dim3((unsigned)((n + 1023) / 1024), P.G), 256, 0, st>>>(P.part, P, P.out, P.out_type, n,
-                                                                                n % 4 == 0 && out_vec(P.out, P.out_type, n));
+      join_units_kernel<<<dim3((unsigned)((n + 2047) / 2048), P.G), 256, 0, st>>>(P.part, P, P.out, P.out_type, n);
     if (P.bsum)
-      join_units_kernel<<<dim3((unsigned)((P.rows_out + 1023) / 1024), P.G), 256, 0, st>>>(
-          P.bsum, P, d->bias_grad, d->bias_type, P.rows_out, P.rows_out % 4 == 0 && out_vec(d->bias_grad, d->bias_type, P.rows_out));
+      join_units_kernel<<<dim3((unsigned)((P.rows_out + 2047) / 2048), P.G), 256, 0, st>>>(P.bsum, P, d->bias_grad, d->bias_type,
+                                                                                         P.rows_out);
   } else if (P.part) {
-    join_rows_kernel<<<dim3((unsigned)((P.cols + 1023) / 1024), (unsigned)(P.S < 32768 ? P.S : 32768)), 256, 0, st>>>(P);
+    join_rows_kernel<<<dim3((unsigned)((P.cols + 2047) / 2048), (unsigned)(P.S < 32768 ? P.S : 32768)), 256, 0, st>>>(P);
   }
   return launch_status();
 }

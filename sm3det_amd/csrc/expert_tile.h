@@ -13,6 +13,9 @@
 //   * The order of the reduction inside an instruction is free as long as both operands agree.
 // Q rides in the instruction's first operand: a lane then owns four CONSECUTIVE output columns of one output row.
 #pragma once
+#include <type_traits>
+#include <utility>
+
 #include "common.h"
 
 namespace sm3x {
@@ -24,6 +27,8 @@ typedef short v4s __attribute__((ext_vector_type(4)));
 typedef short v8s __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef __bf16 v2b __attribute__((ext_vector_type(2)));
 
 enum { DT_F32 = SM3_DT_F32, DT_F16 = SM3_DT_F16, DT_BF16 = SM3_DT_BF16 };
 enum { K_F16 = 0, K_BF16 = 1, K_MX4 = 2 };   // operand kinds
@@ -44,107 +49,177 @@ struct Params {
   long qred;                      // NN: rows of one expert's weights (the reduction length itself)
   void* out;                      // NT / NN: (S, cols).  TN: (G, rows_out, cols)
   int rows_out, cols;             // TN: output rows of one expert; output columns
-  int out_type, bias_type, act, vec;
+  int out_type, bias_type, act;
+  int wide;                       // result rows allow 16-byte stores
+  int bias_lds;                   // bias rows may be loaded as 4-byte words
   const void* bias;               // (G, cols) or null
   float* bsum;                    // TN: per work unit column sums of p (units, rows_out) fp32, or null
   const int* offsets;             // (G + 1) device, or null: one group of all S rows
   int G;
   long S;
   int ntiles;                     // column tiles
-  long mtiles;                    // row tiles the grid provides for (an upper bound where the groups are ragged)
   int splits;                     // NT / NN: slices of the reduction; > 1: fp32 partials (splits, S, cols) in `part`
   long unit_rows;                 // TN: reduction rows per work unit
   float* part;                    // fp32 partials, or null: the result goes straight to `out`
 };
 
-// ---- which rows a tile covers -------------------------------------------------------------------------------------
+// ---- the jobs of a workgroup ----------------------------------------------------------------------------------------
+// A job is one output tile (of one slice of the reduction).  Row tiles are numbered expert by expert; behind them come the
+// tiles of rows that belong to no expert (behind the last, before the first), whose outputs are zero.  Jobs run in bands of 4 row
+// tiles; consecutive jobs run on one XCD (they share operands in its L2).
 // The experts' row ranges are read from the device offsets: clamped to [0, S] and made monotone (running maximum), so that no
-// content of the array can lead an access out of range.  Tiles are numbered expert by expert; behind them come the rows that
-// belong to no expert (before the first, behind the last), whose outputs are zero.
-struct RowTile {
-  int g;           // expert, -1: rows of no expert, -2: nothing to do
-  long row0;
-  int rows;
-  int part_of_g;   // index of this tile within its expert
+// content of the array can lead an access out of range.
+struct Job {
+  int g, row0, rows;  // expert (-1: rows of no expert); NT / NN: output rows.  TN: reduction rows
+  int col0, prow0;    // first output column; TN: first output row
+  int unit;           // slice (NT / NN) or work unit (TN) the result belongs to
+  int s0, s1;         // steps
 };
+constexpr int kMaxJobs = 64;  // of one workgroup: lane l of every wave holds job l
 
-template <bool KEEP_EMPTY>  // KEEP_EMPTY: an expert without rows still gets one unit (its gradient is zero)
-__device__ __forceinline__ RowTile find_rows(const Params& P, long tile, int bm) {
-  RowTile t{-2, 0, 0, 0};
-  if (P.offsets == nullptr) {
-    const long r0 = tile * bm;
-    if (r0 < P.S || (KEEP_EMPTY && tile == 0)) {
-      t.g = 0;
-      t.row0 = r0;
-      t.rows = (int)((P.S - r0 < bm) ? P.S - r0 : bm);
-      t.part_of_g = (int)tile;
+struct Jobs {
+  int g, row0, rows, col0, prow0, unit;  // of this lane's job
+  int count;
+
+  // BM, BN: output tile; row tiles are BM rows (NT / NN) or a work unit of unit_rows reduction rows (TN) with `mper` tiles each
+  template <bool TN, int BM, int BN>
+  __device__ __forceinline__ void init(const Params& P) {
+    const int bm = TN ? (int)P.unit_rows : BM;
+    const unsigned mper = TN ? (unsigned)(P.rows_out + BM - 1) / BM : 1u;  // TN: row tiles of a unit
+    const int lane = threadIdx.x & 63, S = (int)P.S;
+    const auto clamp = [&](int v) { return v < 0 ? 0 : v > S ? S : v; };
+    const auto tiles_of = [&](int len) { const int n = (len + bm - 1) / bm; return TN && n == 0 ? 1 : n; };
+    const auto ends_from = [&](int e) { return P.offsets ? P.offsets[1 + (e + lane < P.G ? e + lane : 0)] : S; };
+    int ends = ends_from(0);
+    const int raw = P.offsets ? P.offsets[0] : 0;
+    const int first = clamp(__builtin_amdgcn_readfirstlane(raw));
+    int last = first, owned = 0;  // rows and row tiles of experts
+    for (int e = 0; e < P.G; e++) {
+      if (e && (e & 63) == 0) ends = ends_from(e);
+      const int end = clamp(__builtin_amdgcn_readlane(ends, e & 63));
+      const int to = end > last ? end : last;
+      owned += tiles_of(to - last);
+      last = to;
     }
-    return t;
+    const int behind = TN ? 0 : (S - last + bm - 1) / bm, before = TN ? 0 : (first + bm - 1) / bm;
+    const unsigned ntiles = (unsigned)P.ntiles, mtiles = (unsigned)(owned + behind + before);
+    const unsigned stride = gridDim.x / kNumXCD, xcd = blockIdx.x % kNumXCD, slot = blockIdx.x / kNumXCD;
+    unsigned t;
+    if constexpr (!TN) {
+      const unsigned tiles = mtiles * ntiles, jobs = tiles * (unsigned)P.splits;
+      const unsigned per = (jobs + kNumXCD - 1) / kNumXCD;
+      const unsigned begin = xcd * per, limit = begin + per < jobs ? begin + per : jobs;
+      const unsigned mine = begin + slot, job = mine + lane * stride;
+      count = mine < limit ? (int)((limit - mine + stride - 1) / stride) : 0;  // (<= kMaxJobs: the grid is made for it)
+      const unsigned z = job / tiles, lin = job - z * tiles;  // (lanes behind the last job compute something nobody reads)
+      const unsigned band = lin / (4u * ntiles), in = lin - band * 4u * ntiles;
+      const unsigned left = mtiles - band * 4u, deep = left < 4u ? (left ? left : 1u) : 4u;
+      const unsigned nt = in / deep;
+      t = band * 4u + (in - nt * deep);
+      col0 = (int)(nt * BN);
+      prow0 = 0;
+      unit = (int)z;
+    } else {
+      // Where units are whole experts they differ in length: every XCD gets an eighth of EACH unit's tiles, units follow each
+      // other from the longest to the shortest (up to 64 experts), and every other round of workgroups runs backwards
+      // (16384 rows, 8 experts, 4096 x 1024: 228 -> 156 us).  Units cut to one length stay whole on an XCD, which then reads
+      // their rows once (65536 rows, 1024 x 256: 85 -> 69 us).
+      const unsigned tiles = mper * ntiles;
+      unsigned u, tile;
+      if (P.part == nullptr) {
+        const unsigned per = (tiles + kNumXCD - 1) / kNumXCD, jobs = per * (unsigned)owned;
+        const unsigned job = lane * stride + ((lane & 1) ? stride - 1 - slot : slot);
+        count = (int)((jobs + stride - 1) / stride);
+        u = job / per;
+        tile = xcd * per + (job - u * per);
+        t = job < jobs && tile < tiles ? u : ~0u;  // (position of the unit in the order of work; none)
+      } else {
+        const unsigned jobs = tiles * (unsigned)owned, per = (jobs + kNumXCD - 1) / kNumXCD;
+        const unsigned begin = xcd * per, limit = begin + per < jobs ? begin + per : jobs;
+        const unsigned mine = begin + slot, job = mine + lane * stride;
+        count = mine < limit ? (int)((limit - mine + stride - 1) / stride) : 0;
+        u = job / tiles;
+        tile = job - u * tiles;
+        t = job < limit ? u : ~0u;
+      }
+      const unsigned pt = tile / ntiles;
+      prow0 = (int)(pt * BM);
+      col0 = (int)((tile - pt * ntiles) * BN);
+    }
+    g = -1;
+    row0 = 0;
+    int end_row = 0;
+    if constexpr (TN) {
+      int at = 0, prev = first;
+      if (P.G <= 64) {
+        int from = 0, len = 0, unit0 = 0, rank = 0;  // lane e: expert e
+        for (int e = 0; e < P.G; e++) {
+          const int end = clamp(__builtin_amdgcn_readlane(ends, e)), to = end > prev ? end : prev;
+          if (lane == e) {
+            from = prev;
+            len = to - prev;
+            unit0 = at;
+          }
+          at += tiles_of(to - prev);
+          prev = to;
+        }
+        for (int e = 0; e < P.G; e++) {
+          const int l = __builtin_amdgcn_readlane(len, e);
+          rank += l > len || (l == len && e < lane) ? 1 : 0;
+        }
+        at = 0;
+        for (int r = 0; r < P.G; r++) {
+          const int e = __ffsll(__ballot(rank == r && lane < P.G)) - 1;
+          const int l = __builtin_amdgcn_readlane(len, e), f = __builtin_amdgcn_readlane(from, e);
+          const int u = __builtin_amdgcn_readlane(unit0, e), n = tiles_of(l);
+          if (t != ~0u && (int)t >= at && (int)t < at + n) {
+            g = e;
+            row0 = f + ((int)t - at) * bm;
+            end_row = f + l;
+            unit = u + (int)t - at;
+          }
+          at += n;
+        }
+      } else {
+        ends = ends_from(0);
+        for (int e = 0; e < P.G; e++) {
+          if (e && (e & 63) == 0) ends = ends_from(e);
+          const int end = clamp(__builtin_amdgcn_readlane(ends, e & 63));
+          const int to = end > prev ? end : prev, n = tiles_of(to - prev);
+          if (t != ~0u && (int)t >= at && (int)t < at + n) {
+            g = e;
+            row0 = prev + ((int)t - at) * bm;
+            end_row = to;
+            unit = (int)t;
+          }
+          at += n;
+          prev = to;
+        }
+      }
+    } else {
+      const int i = (int)t - owned;
+      row0 = i < behind ? last + i * bm : (i - behind) * bm;
+      end_row = i < behind ? S : first;
+      int at = 0, prev = first;
+      if (P.G > 64) ends = ends_from(0);
+      for (int e = 0; e < P.G; e++) {
+        if (e && (e & 63) == 0) ends = ends_from(e);
+        const int end = clamp(__builtin_amdgcn_readlane(ends, e & 63));
+        const int to = end > prev ? end : prev, n = tiles_of(to - prev);
+        if ((int)t >= at && (int)t < at + n) {
+          g = e;
+          row0 = prev + ((int)t - at) * bm;
+          end_row = to;
+        }
+        at += n;
+        prev = to;
+      }
+    }
+    rows = end_row - row0;
+    rows = rows < 0 ? 0 : rows > bm ? bm : rows;
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // (nothing of this is in flight when the loader starts to count its own loads)
   }
-  const int lane = threadIdx.x & 63;
-  const int S = (int)P.S;
-  int first = P.offsets[0];
-  first = first < 0 ? 0 : first > S ? S : first;
-  int carry_end = first;
-  long carry_tiles = 0;
-  for (int base = 0; base < P.G; base += 64) {
-    const int g = base + lane;
-    int end = g < P.G ? P.offsets[g + 1] : 0;
-    end = end < 0 ? 0 : end > S ? S : end;
-    end = end < carry_end ? carry_end : end;
-    for (int d = 1; d < 64; d <<= 1) {
-      const int o = __shfl_up(end, d);
-      if (lane >= d && o > end) end = o;
-    }
-    int start = __shfl_up(end, 1);
-    if (lane == 0) start = carry_end;
-    const int len = end - start;
-    int n = g < P.G ? (len + bm - 1) / bm : 0;
-    if (KEEP_EMPTY && g < P.G && n == 0) n = 1;
-    int incl = n;
-    for (int d = 1; d < 64; d <<= 1) {
-      const int o = __shfl_up(incl, d);
-      if (lane >= d) incl += o;
-    }
-    const unsigned long long hit = __ballot(tile - carry_tiles < incl);
-    if (hit) {
-      const int l = __ffsll(hit) - 1;
-      const int before = __shfl(incl - n, l);
-      const int s0 = __shfl(start, l), e0 = __shfl(end, l);
-      const int idx = (int)(tile - carry_tiles) - before;
-      t.g = base + l;
-      t.part_of_g = idx;
-      t.row0 = (long)s0 + (long)idx * bm;
-      const long left = e0 - t.row0;
-      t.rows = (int)(left < bm ? (left < 0 ? 0 : left) : bm);
-      break;
-    }
-    carry_tiles += __shfl(incl, 63);
-    carry_end = __shfl(end, 63);
-  }
-  if (t.g == -2 && !KEEP_EMPTY) {  // rows of no expert
-    long i = tile - carry_tiles;
-    const long behind = ((long)S - carry_end + bm - 1) / bm;
-    long r0 = -1, r1 = 0;
-    if (i < behind) {
-      r0 = carry_end + i * bm;
-      r1 = S;
-    } else if ((i - behind) * bm < first) {
-      r0 = (i - behind) * bm;
-      r1 = first;
-    }
-    if (r0 >= 0) {
-      t.g = -1;
-      t.row0 = r0;
-      t.rows = (int)(r1 - r0 < bm ? r1 - r0 : bm);
-    }
-  }
-  t.g = __builtin_amdgcn_readfirstlane(t.g);
-  t.row0 = (long)__builtin_amdgcn_readfirstlane((int)t.row0);
-  t.rows = __builtin_amdgcn_readfirstlane(t.rows);
-  t.part_of_g = __builtin_amdgcn_readfirstlane(t.part_of_g);
-  return t;
-}
+};
 
 // ---- global -> LDS ------------------------------------------------------------------------------------------------
 __device__ __forceinline__ v4i descriptor(const void* base, long bytes) {
@@ -167,8 +242,14 @@ __device__ __forceinline__ void dma4(unsigned lds, unsigned voff, v4i desc) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
                :: "s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(voff), "s"(desc) : "memory", "m0");
 }
-// this wave's direct loads have landed; after the barrier everybody's have
-__device__ __forceinline__ void wait_and_sync() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// this wave's direct loads have landed and its LDS reads are done; after the barrier everybody's.  (The builtin, not asm: the
+// compiler then knows that its own loads and stores are complete too and inserts no waits for them into the loop.)
+__device__ __forceinline__ void wait_and_sync() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
 __device__ __forceinline__ unsigned lds_address(const void* p) {
   return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
@@ -180,13 +261,15 @@ __device__ __forceinline__ int col_swz(int row, int granules) {
 }
 
 // One operand tile of BX rows (row operand) or BX columns (column operand): 128 * BX bytes of LDS per step, loaded by
-// `waves` waves with BX / 8 / waves instructions each.
+// `waves` waves with N = BX / 8 / waves instructions ("pieces") each.
 template <int BX, bool COL, int WAVES>
 struct Loader {
   static constexpr int N = BX / 8 / WAVES;
   static_assert(BX / 8 % WAVES == 0 && N >= 1, "every wave loads the same number of 1 KB pieces");
   unsigned voff[N];
   int gran;  // row operand: this lane's granule of the step (loop tail)
+  v4i desc;  // of the step being loaded
+  unsigned cut;
 
   __device__ __forceinline__ void init(int wave, int lane, long ld) {
 #pragma unroll
@@ -203,12 +286,13 @@ struct Loader {
       }
     }
   }
-  // left: bytes (row operand) of the reduction that remain from this step on
-  __device__ __forceinline__ void load(unsigned lds, int wave, const char* base, long bytes, long left) const {
-    const v4i d = descriptor(base, bytes);
-    const unsigned cut = (!COL && gran * 16 >= left) ? kOutOfRange : 0u;
-#pragma unroll
-    for (int i = 0; i < N; i++) dma16(lds + (wave * N + i) * 1024, voff[i] | cut, d);
+  // left: bytes (row operand) of the reduction that remain from this step on; bytes <= 0: nothing is read, zeros arrive
+  __device__ __forceinline__ void aim(const char* base, long bytes, long left) {
+    desc = descriptor(base, bytes);
+    cut = (!COL && gran * 16 >= left) ? kOutOfRange : 0u;
+  }
+  __device__ __forceinline__ void piece(unsigned lds, int wave, int i) const {
+    dma16(lds + (wave * N + i) * 1024, COL ? voff[i] : (voff[i] | cut), desc);
   }
 };
 
@@ -252,256 +336,516 @@ __device__ __forceinline__ v4f mma(v4i q, v4i p, v4f c, int qscale, int pscale, 
 }
 
 // ---- epilogue -----------------------------------------------------------------------------------------------------
-__device__ __forceinline__ float gelu(float h) {  // h * Phi(h), erfc by Abramowitz & Stegun 7.1.26 (|error| <= 1.5e-7)
-  const float e = __expf(-0.5f * h * h);
-  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678118654752440f, fabsf(h), 1.0f));
-  float q = fmaf(1.061405429f, t, -1.453152027f);
-  q = fmaf(q, t, 1.421413741f);
-  q = fmaf(q, t, -0.284496736f);
-  q = fmaf(q, t, 0.254829592f);
-  const float tail = 0.5f * q * t * e;  // Phi(-|h|)
-  return h * (h >= 0.f ? 1.0f - tail : tail);
+// GELU(h) = h Phi(h) = max(h, 0) - |h| Phi(-|h|), with Phi(-a) = 2^p(a): log2 Phi(-a) is so smooth that a polynomial of degree 7
+// (fitted here by linear programming on [0, 6], minimax in the error relative to |h|) leaves 3.6e-8 |h|, 1.2e-7 |h| with the
+// fp32 rounding of its evaluation; behind 6 |h| Phi(-|h|) is below 6e-9.  One transcendental instruction and 11 others: with the
+// erfc form of Abramowitz & Stegun 7.1.26 (two and 12, error 1e-7) the epilogue of a 4-bit product was bound by GELU.
+// (h / 2 + |h| / 2 is max(h, 0) that lets a NaN through.)
+// Eight at once, step by step, so that no instruction waits for the one before it.
+__device__ __forceinline__ void gelu8(float (&h)[8]) {
+  constexpr float c[8] = {-0.9999998807907104f,   -1.1511108875274658f, -0.4591531455516815f,    -0.05269111320376396f,
+                          0.007389274425804615f, -0.0004212373751215637f, -5.390329170040786e-05f, 8.470114153169561e-06f};
+  float a[8], p[8];
+#pragma unroll
+  for (int r = 0; r < 8; r++) a[r] = fminf(fabsf(h[r]), 6.0f);
+#pragma unroll
+  for (int r = 0; r < 8; r++) p[r] = fmaf(c[7], a[r], c[6]);
+#pragma unroll
+  for (int k = 5; k >= 0; k--) {
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int r = 0; r < 8; r++) p[r] = fmaf(p[r], a[r], c[k]);
+  }
+#pragma unroll
+  for (int r = 0; r < 8; r++) p[r] = __builtin_amdgcn_exp2f(p[r]);
+#pragma unroll
+  for (int r = 0; r < 8; r++) h[r] = fmaf(-a[r], p[r], fmaf(0.5f, fabsf(h[r]), 0.5f * h[r]));
 }
 
-__device__ __forceinline__ float load_bias(const void* b, int type, long i) {
-  if (type == DT_F32) return ((const float*)b)[i];
-  if (type == DT_F16) return (float)((const _Float16*)b)[i];
-  return (float)((const __bf16*)b)[i];
-}
-
-// four consecutive columns of one row; n: how many of them exist
-__device__ __forceinline__ void store4(void* out, int type, long at, v4f v, int n, bool vec) {
+// the eight values b[at .. at + 7], indexes clamped to `most` (what lies behind is not stored)
+__device__ __forceinline__ void bias8(float (&v)[8], const void* b, int type, long at, long most) {
   if (type == DT_F32) {
-    float* o = (float*)out + at;
-    if (vec && n == 4) *(v4f*)o = v;
-    else
-      for (int r = 0; r < 4; r++) { if (r < n) o[r] = v[r]; }
-  } else if (type == DT_F16) {
-    typedef _Float16 v4h __attribute__((ext_vector_type(4)));
-    _Float16* o = (_Float16*)out + at;
-    const v4h h = __builtin_convertvector(v, v4h);
-    if (vec && n == 4) *(v4h*)o = h;
-    else
-      for (int r = 0; r < 4; r++) { if (r < n) o[r] = h[r]; }
+#pragma unroll
+    for (int r = 0; r < 8; r++) v[r] = ((const float*)b)[at + r < most ? at + r : most];
   } else {
-    typedef __bf16 v4b __attribute__((ext_vector_type(4)));
-    __bf16* o = (__bf16*)out + at;
-    const v4b h = __builtin_convertvector(v, v4b);
-    if (vec && n == 4) *(v4b*)o = h;
-    else
-      for (int r = 0; r < 4; r++) { if (r < n) o[r] = h[r]; }
+    unsigned short h[8];
+#pragma unroll
+    for (int r = 0; r < 8; r++) h[r] = ((const unsigned short*)b)[at + r < most ? at + r : most];
+#pragma unroll
+    for (int r = 0; r < 8; r++)
+      v[r] = type == DT_F16 ? (float)__builtin_bit_cast(_Float16, h[r]) : __uint_as_float((unsigned)h[r] << 16);
   }
 }
 
+// four consecutive ones (a multiple of 4 from the row's start: the row may be read in words), their place clamped to `most`
+__device__ __forceinline__ v4f bias4(const void* b, int type, long at, long most) {
+  at = at < most ? at : most;
+  if (type == DT_F32) {
+    const float* f = (const float*)b + at;
+    return v4f{f[0], f[1], f[2], f[3]};
+  }
+  const unsigned short* u = (const unsigned short*)b + at;
+  unsigned short h[4];
+#pragma unroll
+  for (int r = 0; r < 4; r++) h[r] = u[r];
+  v4f v;
+#pragma unroll
+  for (int r = 0; r < 4; r++) v[r] = type == DT_F16 ? (float)__builtin_bit_cast(_Float16, h[r]) : __uint_as_float((unsigned)h[r] << 16);
+  return v;
+}
+
+__device__ __forceinline__ unsigned pack2(float a, float b, int type) {  // rounded to nearest even
+  if (type == DT_F16) {
+    const _Float16 x = (_Float16)a, y = (_Float16)b;
+    return (unsigned)__builtin_bit_cast(unsigned short, x) | (unsigned)__builtin_bit_cast(unsigned short, y) << 16;
+  }
+  const __bf16 x = (__bf16)a, y = (__bf16)b;
+  return (unsigned)__builtin_bit_cast(unsigned short, x) | (unsigned)__builtin_bit_cast(unsigned short, y) << 16;
+}
+
+// eight consecutive values of one row, `n` of them exist; wide: 16-byte stores are allowed (and n is a multiple of what one holds)
+__device__ __forceinline__ void store8(void* out, int type, long at, const float (&v)[8], int n, bool wide) {
+  if (type == DT_F32) {
+    float* o = (float*)out + at;
+    if (wide) {
+      if (n >= 4) *(v4f*)o = v4f{v[0], v[1], v[2], v[3]};
+      if (n >= 8) *(v4f*)(o + 4) = v4f{v[4], v[5], v[6], v[7]};
+    } else {
+#pragma unroll
+      for (int r = 0; r < 8; r++) { if (r < n) o[r] = v[r]; }
+    }
+    return;
+  }
+  v8s h;
+  if (type == DT_F16) {
+#pragma unroll
+    for (int r = 0; r < 8; r++) h[r] = __builtin_bit_cast(short, (_Float16)v[r]);
+  } else {
+#pragma unroll
+    for (int r = 0; r < 8; r++) h[r] = __builtin_bit_cast(short, (__bf16)v[r]);
+  }
+  short* o = (short*)out + at;
+  if (wide) *(v8s*)o = h;
+  else {
+#pragma unroll
+    for (int r = 0; r < 8; r++) { if (r < n) o[r] = h[r]; }
+  }
+}
+
+template <int... I, class F>
+__device__ __forceinline__ void for_each_of(std::integer_sequence<int, I...>, F f) { (f(std::integral_constant<int, I>{}), ...); }
+template <int N, class F>
+__device__ __forceinline__ void for_each(F f) { for_each_of(std::make_integer_sequence<int, N>{}, f); }
+
 // ---- the kernel ---------------------------------------------------------------------------------------------------
-// BM output rows (P) x BN output columns (Q); WM x WN waves.
-template <int KIND, int MODE, int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(WM * WN * 64) tile_kernel(const Params P) {
-  constexpr int WAVES = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
+// BM output rows (P) x BN output columns (Q); WM x WN waves, MINW waves per SIMD.
+//
+// A workgroup runs through a list of tiles (jobs) as ONE sequence of steps: the loader is two steps ahead of the matrix unit and
+// walks into the next tile while the current one is finished and stored, so a tile costs neither a ramp nor a drain.
+// Two LDS buffers, one barrier per step.  A step is two rounds; while the matrix unit works on one round's fragments, the
+// next round's are read from LDS, piece by piece between the instructions (round 1 reads round 0 of the NEXT step, so the
+// barrier stands between the rounds: by then this step's buffer has been read out and the next one has landed):
+//     round 0: multiply f0 | read f1 from buffer i
+//     wait for the loads of step i + 1 (issued a whole step ago), barrier
+//     round 1: multiply f1 | read f0 from buffer i + 1 | start loading step i + 2 into buffer i
+template <int KIND, int MODE, int BM, int BN, int WM, int WN, int MINW>
+__global__ void __launch_bounds__(WM * WN * 64, MINW) tile_kernel(const Params P) {
+  constexpr int WAVES = WM * WN, TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
   constexpr bool PCOL = MODE == M_TN, QCOL = MODE != M_NT;
   static_assert(KIND != K_MX4 || MODE == M_NT, "4-bit operands: rows only");
+  constexpr bool ACT = KIND == K_MX4;  // (the 16-bit products have no activation: their gradients would need its derivative)
   constexpr int kTile = (BM + BN) * kStepBytes;
-  constexpr int kScales = KIND == K_MX4 ? (BM + BN) * 8 : 0;
-  __shared__ __attribute__((aligned(1024))) char lds[2][kTile + kScales];
+  constexpr int NS = KIND == K_MX4 ? ((BM + BN) / 32 + WAVES - 1) / WAVES : 0;  // scale pieces of a wave: 32 rows x 8 bytes each
+  constexpr int kScales = NS * WAVES * 256;
+  constexpr int kBuf = kTile + kScales;
+  constexpr int kStage = 8 * (TN * 4 + 16);  // epilogue: 8 rows of a wave's columns
+  constexpr int kBias = MODE == M_TN ? 0 : 4 * BN * 4 + 256;  // bias rows of four jobs (the loader is at most two ahead)
+  __shared__ __attribute__((aligned(1024))) char lds[2 * kBuf + WAVES * kStage + kBias];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % WM, wn = wave / WM;
 
-  // tile of this workgroup: consecutive tiles on one XCD (they share weights in its L2), bands of 4 row tiles
-  const long total = P.mtiles * P.ntiles;
-  const long per = (total + kNumXCD - 1) / kNumXCD;
-  const long lin = (long)(blockIdx.x % kNumXCD) * per + blockIdx.x / kNumXCD;
-  if (lin >= total || (long)(blockIdx.x / kNumXCD) >= per) return;
-  const long band = lin / (4L * P.ntiles), in = lin % (4L * P.ntiles);
-  const long left = P.mtiles - band * 4;
-  const int deep = left < 4 ? (int)left : 4;
-  const int nt = (int)(in / deep);
-  const long mt = band * 4 + in % deep;
+  Jobs jobs;
+  jobs.init<MODE == M_TN, BM, BN>(P);
+  const int red_steps = MODE == M_TN ? 0 : (int)((P.red + kStepBytes - 1) / kStepBytes);
+  const int slice = MODE == M_TN ? 0 : (red_steps + P.splits - 1) / P.splits;
+  auto job_of = [&](int j) {
+    Job w;
+    w.g = __builtin_amdgcn_readlane(jobs.g, j);
+    w.row0 = __builtin_amdgcn_readlane(jobs.row0, j);
+    w.rows = __builtin_amdgcn_readlane(jobs.rows, j);
+    w.col0 = __builtin_amdgcn_readlane(jobs.col0, j);
+    w.prow0 = __builtin_amdgcn_readlane(jobs.prow0, j);
+    w.unit = __builtin_amdgcn_readlane(jobs.unit, j);
+    if constexpr (MODE == M_TN) {
+      w.s0 = 0;
+      w.s1 = (w.rows + kStepRed - 1) / kStepRed;
+    } else {
+      const int steps = w.g < 0 ? 0 : red_steps, a = w.unit * slice;
+      w.s0 = a < steps ? a : steps;
+      w.s1 = w.s0 + slice < steps ? w.s0 + slice : steps;
+    }
+    return w;
+  };
 
-  long red_steps, row0 = 0, prow0 = 0;
-  int rows, g, mtile = 0;
-  RowTile t;
-  if constexpr (MODE == M_TN) {
-    const int mt_per_unit = (P.rows_out + BM - 1) / BM;
-    t = find_rows<true>(P, mt / mt_per_unit, (int)P.unit_rows);
-    if (t.g < 0) return;
-    g = t.g;
-    mtile = (int)(mt % mt_per_unit);
-    prow0 = (long)mtile * BM;
-    rows = t.rows;                      // reduction rows
-    red_steps = (rows + kStepRed - 1) / kStepRed;
-  } else {
-    t = find_rows<false>(P, mt, BM);
-    if (t.g == -2) return;
-    g = t.g;
-    row0 = t.row0;
-    rows = t.rows;
-    red_steps = g < 0 ? 0 : (P.red + kStepBytes - 1) / kStepBytes;
-  }
-  const long col0 = (long)nt * BN;
-
-  // this slice of the reduction
-  long step0 = 0, step1 = red_steps;
-  if (MODE != M_TN && P.splits > 1) {
-    const long each = (red_steps + P.splits - 1) / P.splits;
-    step0 = blockIdx.y * each;
-    step1 = step0 + each < red_steps ? step0 + each : red_steps;
-    if (step0 > step1) step0 = step1;
-  }
-
+  // ---- the loader
   Loader<BM, PCOL, WAVES> lp;
   Loader<BN, QCOL, WAVES> lq;
   lp.init(wave, lane, P.ldp);
   lq.init(wave, lane, P.ldq);
-  const unsigned base = __builtin_amdgcn_readfirstlane((int)lds_address(&lds[0][0]));
+  constexpr int ND = lp.N + lq.N + NS;
+  const unsigned base = __builtin_amdgcn_readfirstlane((int)lds_address(lds));
+  char* const bias_lds = lds + 2 * kBuf + WAVES * kStage;
 
-  const int qrows = (int)(P.cols - col0 < BN ? P.cols - col0 : BN);
-  auto load_step = [&](long it, int buf) {
-    const unsigned at = base + buf * (kTile + kScales);
-    if constexpr (!PCOL) {
-      const long k = it * kStepBytes;
-      lp.load(at, wave, P.p + row0 * P.ldp + k, (long)(rows - 1) * P.ldp + P.red - k, P.red - k);
-    } else {
-      const long r = it * kStepRed, n = rows - r < kStepRed ? rows - r : kStepRed;
-      const long wide = ((long)P.rows_out * 2 + 15) & ~15L;
-      lp.load(at, wave, P.p + (t.row0 + r) * P.ldp + prow0 * 2, (n - 1) * P.ldp + wide - prow0 * 2, 0);
-    }
-    const unsigned qa = at + BM * kStepBytes;
-    if constexpr (MODE == M_NT) {
-      const long k = it * kStepBytes;
-      lq.load(qa, wave, P.q + g * P.strideq + col0 * P.ldq + k, (long)(qrows - 1) * P.ldq + P.red - k, P.red - k);
-    } else {
-      const long wide = ((long)P.cols * 2 + 15) & ~15L;
-      const long r = it * kStepRed;
-      long n, first;
-      const char* q;
-      if constexpr (MODE == M_NN) {
-        n = P.qred - r;
-        q = P.q + g * P.strideq;
-        first = r;
-      } else {
-        n = rows - r;
-        q = P.q;
-        first = t.row0 + r;
+  int lj = 0, lit = 0, lnum = -1;  // job being loaded, its step, its ordinal among the jobs that load anything
+  Job lw{};
+  bool more = true;
+  const char *pb = P.p, *qb = P.q;                 // where the step starts
+  const unsigned char *psb = P.ps, *qsb = P.qs;    // MX4: scale bytes
+  int kleft = 0, rleft = 0;                        // row operand: bytes, column operand: rows of the reduction that remain
+  auto enter = [&]() {  // the first job from lj on that has steps
+    for (;; lj++) {
+      if (lj >= jobs.count) {
+        more = false;
+        return;
       }
-      if (n > kStepRed) n = kStepRed;
-      lq.load(qa, wave, q + first * P.ldq + col0 * 2, (n - 1) * P.ldq + wide - col0 * 2, 0);
+      lw = job_of(lj);
+      if (lw.s0 < lw.s1) break;
     }
-    if constexpr (KIND == K_MX4) {  // 8 scale bytes per row and step: 32 rows per instruction
-      const unsigned sa = at + kTile;
-      const long kb = it * 8, most = P.red / 16;  // scale bytes of a row
+    lit = lw.s0;
+    lnum++;
+    const long k = (long)lit * kStepBytes, r = (long)lit * kStepRed;
+    if constexpr (MODE == M_TN) {
+      pb = P.p + (lw.row0 + r) * P.ldp + (long)lw.prow0 * 2;
+      qb = P.q + (lw.row0 + r) * P.ldq + (long)lw.col0 * 2;
+      rleft = lw.rows - (int)r;
+    } else {
+      pb = P.p + (long)lw.row0 * P.ldp + k;
+      kleft = (int)(P.red - k);
+      if constexpr (MODE == M_NN) {
+        qb = P.q + lw.g * P.strideq + r * P.ldq + (long)lw.col0 * 2;
+        rleft = (int)(P.qred - r);
+      } else {
+        qb = P.q + lw.g * P.strideq + (long)lw.col0 * P.ldq + k;
+      }
+    }
+    if constexpr (KIND == K_MX4) {
+      psb = P.ps + (long)lw.row0 * P.ldps + lit * 8;
+      qsb = P.qs + lw.g * P.strideqs + (long)lw.col0 * P.ldqs + lit * 8;
+    }
+  };
+  auto aim = [&]() {  // descriptors of the step at (lw, lit); nothing is left: empty ones (zeros arrive)
+    const int qrows = P.cols - lw.col0 < BN ? P.cols - lw.col0 : BN;
+    const int n = rleft < kStepRed ? rleft : kStepRed;
+    const int pw = (P.rows_out * 2 + 15) & ~15, qw = (P.cols * 2 + 15) & ~15;
+    if constexpr (PCOL) lp.aim(pb, more ? (n - 1) * (int)P.ldp + pw - lw.prow0 * 2 : 0, 0);
+    else lp.aim(pb, more ? (lw.rows - 1) * (int)P.ldp + kleft : 0, kleft);
+    if constexpr (QCOL) lq.aim(qb, more ? (n - 1) * (int)P.ldq + qw - lw.col0 * 2 : 0, 0);
+    else lq.aim(qb, more ? (qrows - 1) * (int)P.ldq + kleft : 0, kleft);
+  };
+  // scale pieces (no branches here: they would tear the rounds' instructions apart)
+  unsigned svoff[NS ? NS : 1], scut = 0;
+  v4i sdesc[NS ? NS : 1];
+  if constexpr (KIND == K_MX4) {
 #pragma unroll
-      for (int c = 0; c < ((BM + BN) / 32 + WAVES - 1) / WAVES; c++) {
-        const int i = c * WAVES + wave;
-        if (i >= (BM + BN) / 32) break;
-        const bool isp = i < BM / 32;
-        const int row = (isp ? i : i - BM / 32) * 32 + (lane >> 1);
-        const long ld = isp ? P.ldps : P.ldqs;
-        const char* b = (const char*)(isp ? P.ps + row0 * P.ldps : P.qs + g * P.strideqs + col0 * P.ldqs) + kb;
-        const int n = isp ? rows : qrows;
-        const unsigned cut = kb + 4 * (lane & 1) >= most ? kOutOfRange : 0u;
-        dma4(sa + i * 256, ((unsigned)(row * ld) + 4 * (lane & 1)) | cut, descriptor(b, (long)(n - 1) * ld + most - kb));
+    for (int c = 0; c < NS; c++) {
+      const int i = c * WAVES + wave, row = (i < BM / 32 ? i : i - BM / 32) * 32 + (lane >> 1);
+      svoff[c] = (unsigned)(row * (int)(i < BM / 32 ? P.ldps : P.ldqs)) + 4 * (lane & 1);
+    }
+  }
+  auto aim_scales = [&]() {
+    if constexpr (KIND == K_MX4) {
+      const int have = kleft / 16, qrows = P.cols - lw.col0 < BN ? P.cols - lw.col0 : BN;
+      const int pbytes = (lw.rows - 1) * (int)P.ldps + have, qbytes = (qrows - 1) * (int)P.ldqs + have;
+      scut = 4 * (lane & 1) >= have ? kOutOfRange : 0u;
+#pragma unroll
+      for (int c = 0; c < NS; c++) {
+        const int i = c * WAVES + wave;  // (pieces behind the last read nothing; their zeros go to padding)
+        const int bytes = i < BM / 32 ? pbytes : i < (BM + BN) / 32 ? qbytes : 0;
+        sdesc[c] = descriptor(i < BM / 32 ? psb : qsb, more ? bytes : 0);
+      }
+    }
+  };
+  auto dma = [&](unsigned at, int d) {  // piece d of the step aimed at, into the buffer at LDS address `at`
+    if (d < lp.N) lp.piece(at, wave, d);
+    else if (d < lp.N + lq.N) lq.piece(at + BM * kStepBytes, wave, d - lp.N);
+    else if constexpr (KIND == K_MX4) {  // 8 scale bytes per row and step: 32 rows per instruction
+      const int c = d - lp.N - lq.N;
+      dma4(at + kTile + (c * WAVES + wave) * 256, svoff[c] | scut, sdesc[c]);
+    }
+  };
+  auto advance = [&]() {  // to the next step (of the next job where this one ends)
+    if (!more) return;
+    if (++lit >= lw.s1) {
+      lj++;
+      enter();
+    } else {
+      if constexpr (PCOL) pb += kStepRed * P.ldp; else pb += kStepBytes;
+      if constexpr (QCOL) qb += kStepRed * P.ldq; else qb += kStepBytes;
+      kleft -= kStepBytes;
+      rleft -= kStepRed;
+      if constexpr (KIND == K_MX4) {
+        psb += 8;
+        qsb += 8;
+      }
+    }
+  };
+  // the bias row of a job travels with its first step as one more piece (slot: the job's ordinal modulo 4; other steps load
+  // nothing into a fifth)
+  const int bes = P.bias_type == DT_F32 ? 4 : 2;
+  unsigned bias_to = 0;
+  v4i bdesc = {};
+  auto aim_bias = [&]() {
+    if constexpr (MODE != M_TN) {
+      const bool now = P.bias_lds && more && lit == lw.s0 && wave * 256 < BN * bes;
+      const long at = ((long)lw.g * P.cols + lw.col0) * bes;
+      bdesc = descriptor((const char*)P.bias + at, now ? (long)(P.cols - lw.col0) * bes : 0);
+      bias_to = base + (unsigned)(bias_lds - lds) + (now ? (lnum & 3) * (BN * 4) + wave * 256 : 4 * (BN * 4));
+    }
+  };
+  auto dma_bias = [&]() {
+    if constexpr (MODE != M_TN) dma4(bias_to, wave * 256 + lane * 4, bdesc);
+  };
+  static_assert(MODE == M_TN || WAVES * 256 >= BN * 4, "one bias piece per wave");
+
+  // ---- fragments (and scale pairs) of the two rounds
+  v4i fp[2][FM], fq[2][FN];
+  int ps[2][FM] = {}, qs[2][FN] = {};  // [1]: of the next step, read with its round 0
+  constexpr int NR = FM + FN;
+  auto read = [&](const char* buf, int s, int r) {  // fragment r of round s
+    if (r < FN) {
+      if constexpr (QCOL) fq[s][r] = frag_col<BN>(buf + BM * kStepBytes, wn * TN + r * 16, s, lane);
+      else fq[s][r] = frag_row<KIND>(buf + BM * kStepBytes, wn * TN + r * 16, s, lane);
+    } else {
+      const int i = r - FN;
+      if constexpr (PCOL) fp[s][i] = frag_col<BM>(buf, wm * TM + i * 16, s, lane);
+      else fp[s][i] = frag_row<KIND>(buf, wm * TM + i * 16, s, lane);
+    }
+  };
+  auto read_scale = [&](const char* buf, int set, int r) {
+    const char* ts = buf + kTile + 2 * (lane >> 4) + (lane & 15) * 8;
+    if (r < FN) qs[set][r] = *(const unsigned short*)(ts + (BM + wn * TN + r * 16) * 8);
+    else ps[set][r - FN] = *(const unsigned short*)(ts + (wm * TM + (r - FN) * 16) * 8);
+  };
+
+  v4f acc[FM][FN];
+  float bacc[FM];  // TN: column sums of p (tiles of the first columns), this lane's share of the reduction
+  bool sums = false;
+  // round s: multiply; at even distances issue the NR reads of the other round and (round 1) the ND pieces
+  auto round = [&](auto S, const char* next, unsigned into) {
+    constexpr int s = decltype(S)::value;
+    constexpr int T = FM * FN;
+#pragma unroll
+    for (int q = 0; q < T; q++) {
+      const int i = q / FN, j = q % FN;
+#pragma unroll
+      for (int r = q * NR / T; r < (q + 1) * NR / T; r++) {
+        read(next, s ^ 1, r);
+        if constexpr (KIND == K_MX4 && s == 1) read_scale(next, 1, r);
+      }
+      if constexpr (s == 1) {
+#pragma unroll
+        for (int d = q * ND / T; d < (q + 1) * ND / T; d++) dma(into, d);
+        if (q == T / 2) dma_bias();
+      }
+      acc[i][j] = mma<KIND>(fq[s][j], fp[s][i], acc[i][j], qs[0][j], ps[0][i], s);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (MODE == M_TN) {
+      if (sums) {
+#pragma unroll
+        for (int i = 0; i < FM; i++)
+#pragma unroll
+          for (int h = 0; h < 4; h++) {
+            const int two = fp[s][i][h];  // (a value of its own: a bit cast of the vector's element itself reads element 0)
+            if constexpr (KIND == K_F16)
+              bacc[i] = __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, two), __builtin_bit_cast(v2h, 0x3c003c00), bacc[i], false);
+            else
+              bacc[i] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2b, two), __builtin_bit_cast(v2b, 0x3f803f80), bacc[i],
+                                                        false);
+          }
       }
     }
   };
 
-  v4f acc[FM][FN];
+  enter();
+  if (more) {
+    aim();
+    aim_scales();
 #pragma unroll
-  for (int i = 0; i < FM; i++)
+    for (int d = 0; d < ND; d++) dma(base, d);
+    aim_bias();
+    dma_bias();
+    advance();
+    aim();
+    aim_scales();
 #pragma unroll
-    for (int j = 0; j < FN; j++) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
-  v4f bacc[FM];  // TN: column sums of p, by a product with ones (workgroups of the first column tile)
-#pragma unroll
-  for (int i = 0; i < FM; i++) bacc[i] = v4f{0.f, 0.f, 0.f, 0.f};
-  const bool sums = MODE == M_TN && P.bsum != nullptr && nt == 0 && wn == 0;
-
-  if (step0 < step1) load_step(step0, 0);
-  for (long it = step0; it < step1; it++) {
-    const int buf = (int)(it - step0) & 1;
+    for (int d = 0; d < ND; d++) dma(base + kBuf, d);
+    aim_bias();
+    dma_bias();
     wait_and_sync();
-    if (it + 1 < step1) load_step(it + 1, buf ^ 1);
-    const char* tp = lds[buf];
-    const char* tq = lds[buf] + BM * kStepBytes;
-    int ps[FM] = {}, qs[FN] = {};
-    if constexpr (KIND == K_MX4) {
-      const char* ts = lds[buf] + kTile;
 #pragma unroll
-      for (int i = 0; i < FM; i++)
-        ps[i] = *(const unsigned short*)(ts + (wm * (BM / WM) + i * 16 + (lane & 15)) * 8 + 2 * (lane >> 4));
-#pragma unroll
-      for (int j = 0; j < FN; j++)
-        qs[j] = *(const unsigned short*)(ts + (BM + wn * (BN / WN) + j * 16 + (lane & 15)) * 8 + 2 * (lane >> 4));
+    for (int r = 0; r < NR; r++) {
+      read(lds, 0, r);
+      if constexpr (KIND == K_MX4) read_scale(lds, 0, r);
     }
+  }
+
+  unsigned off = 0;
+  int num = -1;
+  for (int cj = 0; cj < jobs.count; cj++) {
+    const Job w = job_of(cj);
+    if (MODE == M_TN && w.g < 0) continue;  // (the XCDs' shares of a unit's tiles are rounded up)
 #pragma unroll
-    for (int s = 0; s < 2; s++) {
-      v4i fq[FN], fp[FM];
+    for (int i = 0; i < FM; i++)
 #pragma unroll
-      for (int j = 0; j < FN; j++) {
-        if constexpr (QCOL) fq[j] = frag_col<BN>(tq, wn * (BN / WN) + j * 16, s, lane);
-        else fq[j] = frag_row<KIND>(tq, wn * (BN / WN) + j * 16, s, lane);
+      for (int j = 0; j < FN; j++) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+    if constexpr (MODE == M_TN) {
+      sums = P.bsum != nullptr && w.col0 == 0 && wn == 0;
+#pragma unroll
+      for (int i = 0; i < FM; i++) bacc[i] = 0.f;
+    }
+    if (w.s0 < w.s1) num++;
+    for (int it = w.s0; it < w.s1; it++) {
+      // (everything with branches stands before the rounds: the multiplications are free of side effects, and the compiler
+      // would move those of a round behind a branch that follows it, away from the loads they are to cover)
+      advance();
+      aim();
+      aim_scales();
+      aim_bias();
+      __builtin_amdgcn_sched_barrier(0);
+      round(std::integral_constant<int, 0>{}, lds + off, 0);
+      wait_and_sync();
+      __builtin_amdgcn_sched_barrier(0);
+      round(std::integral_constant<int, 1>{}, lds + (kBuf - off), base + off);
+      if constexpr (KIND == K_MX4) {
+#pragma unroll
+        for (int j = 0; j < FN; j++) qs[0][j] = qs[1][j];
+#pragma unroll
+        for (int i = 0; i < FM; i++) ps[0][i] = ps[1][i];
       }
+      off = kBuf - off;
+    }
+
+    int lane = threadIdx.x & 63;  // (opaque: what follows is computed here and not kept in registers through the loop)
+    asm volatile("" : "+v"(lane));
+    // ---- the tile is complete: a lane holds columns 4 (lane / 16) .. + 3 of output row lane % 16 of every 16 x 16 block
+    if (MODE == M_TN && sums) {
 #pragma unroll
       for (int i = 0; i < FM; i++) {
-        if constexpr (PCOL) fp[i] = frag_col<BM>(tp, wm * (BM / WM) + i * 16, s, lane);
-        else fp[i] = frag_row<KIND>(tp, wm * (BM / WM) + i * 16, s, lane);
-      }
-#pragma unroll
-      for (int i = 0; i < FM; i++)
-#pragma unroll
-        for (int j = 0; j < FN; j++) acc[i][j] = mma<KIND>(fq[j], fp[i], acc[i][j], qs[j], ps[i], s);
-      if constexpr (MODE == M_TN) {
-        if (sums) {
-          const int one = KIND == K_F16 ? 0x3c003c00 : 0x3f803f80;
-          const v4i ones = {one, one, one, one};
-#pragma unroll
-          for (int i = 0; i < FM; i++) bacc[i] = mma<KIND>(ones, fp[i], bacc[i], 0, 0, s);
-        }
+        float v = bacc[i];  // the four lane groups hold different reduction rows of the same column
+        v += __shfl_xor(v, 16);
+        v += __shfl_xor(v, 32);
+        const int orow = w.prow0 + wm * TM + i * 16 + lane;
+        if (lane < 16 && orow < P.rows_out) P.bsum[(long)w.unit * P.rows_out + orow] = v;
       }
     }
-  }
-
-  // a lane holds columns 4 (lane / 16) .. + 3 of output row lane % 16 of every 16 x 16 block
-  const long unit = MODE == M_TN ? mt / ((P.rows_out + BM - 1) / BM) : 0;
+    void* const out = P.part ? (void*)P.part : P.out;
+    const int type = P.part ? DT_F32 : P.out_type;
+    const long first = P.part ? (MODE == M_TN ? (long)w.unit * P.rows_out : (long)w.unit * P.S)
+                              : (MODE == M_TN ? (long)w.g * P.rows_out : 0L);
+    const int orow0 = (MODE == M_TN ? w.prow0 : w.row0) + wm * TM;       // first output row of the wave ...
+    const int olim = MODE == M_TN ? P.rows_out : w.row0 + w.rows;        // ... and the end of the rows the tile may write
+    const bool finish = MODE != M_TN && P.part == nullptr && w.g >= 0;
+    if (P.wide) {
+      // Straight from the accumulators.  fp32: a lane's four columns are one 16-byte store.  16 bits: two neighbouring blocks
+      // (j, j + 1) are exchanged between the 16-lane rows (v_permlane16_swap: odd rows of the one with even rows of the
+      // other), which leaves every lane eight consecutive columns; a store instruction covers 64 contiguous bytes of 16 rows.
+      v4f bias[FN];
+      const int bcol = wn * TN + 4 * (lane >> 4);
 #pragma unroll
-  for (int i = 0; i < FM; i++) {
-    const int m = wm * (BM / WM) + i * 16 + (lane & 15);
-    if constexpr (MODE == M_TN) {
-      const long orow = prow0 + m;
-      if (orow >= P.rows_out) continue;
-      if (sums && lane < 16) P.bsum[unit * P.rows_out + orow] = bacc[i][0];
+      for (int j = 0; j < FN; j++) bias[j] = v4f{0.f, 0.f, 0.f, 0.f};
+      if (MODE != M_TN && finish && P.bias) {
+        if (P.bias_lds) {
 #pragma unroll
-      for (int j = 0; j < FN; j++) {
-        const long n = col0 + wn * (BN / WN) + j * 16 + 4 * (lane >> 4);
-        const int have = (int)(P.cols - n < 4 ? P.cols - n : 4);
-        if (have <= 0) continue;
-        if (P.part) store4(P.part, DT_F32, (unit * P.rows_out + orow) * P.cols + n, acc[i][j], have, P.cols % 4 == 0);
-        else store4(P.out, P.out_type, ((long)g * P.rows_out + orow) * P.cols + n, acc[i][j], have, P.vec);
-      }
-    } else {
-      if (m >= rows) continue;
-      const long orow = row0 + m;
+          for (int j = 0; j < FN; j++) bias[j] = bias4(bias_lds + (num & 3) * (BN * 4), P.bias_type, bcol + j * 16, BN - 4);
+          __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+        } else {
+          const long at = (long)w.g * P.cols;
 #pragma unroll
-      for (int j = 0; j < FN; j++) {
-        const long n = col0 + wn * (BN / WN) + j * 16 + 4 * (lane >> 4);
-        const int have = (int)(P.cols - n < 4 ? P.cols - n : 4);
-        if (have <= 0) continue;
-        v4f v = acc[i][j];
-        if (P.part) {
-          store4(P.part, DT_F32, ((long)blockIdx.y * P.S + orow) * P.cols + n, v, have, P.cols % 4 == 0);
-          continue;
+          for (int j = 0; j < FN; j++) bias[j] = bias4(P.bias, P.bias_type, at + w.col0 + bcol + j * 16, at + P.cols - 4);
+          __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
         }
-        if (g >= 0) {
+        // waited for here, on this path: left to the first use, the compiler puts a wait for EVERY load into the next tile's loop
+      }
+      const int g16 = lane >> 4, ncol = w.col0 + wn * TN;
+      for_each<FM>([&](auto I) {  // (the accumulators are registers: their indexes have to be constants)
+        constexpr int i = decltype(I)::value;
+        if (orow0 + i * 16 >= olim) return;
+        const int orow = orow0 + i * 16 + (lane & 15);
+        char* const row = (char*)out + (first + orow) * P.cols * (type == DT_F32 ? 4 : 2);
+#pragma unroll
+        for (int j = 0; j < FN; j += 2) {
+          float v[8];
 #pragma unroll
           for (int r = 0; r < 4; r++) {
-            if (P.bias && r < have) v[r] += load_bias(P.bias, P.bias_type, (long)g * P.cols + n + r);
-            if (P.act) v[r] = gelu(v[r]);
+            v[r] = acc[i][j][r] + bias[j][r];
+            v[r + 4] = acc[i][j + 1][r] + bias[j + 1][r];
+          }
+          if (ACT && finish && P.act) gelu8(v);
+          if (type == DT_F32) {
+            const int n = ncol + j * 16 + 4 * g16;
+            if (orow < olim && n < P.cols) *(v4f*)(row + n * 4) = v4f{v[0], v[1], v[2], v[3]};
+            if (orow < olim && n + 16 < P.cols) *(v4f*)(row + n * 4 + 64) = v4f{v[4], v[5], v[6], v[7]};
+          } else {
+            unsigned h[4];
+#pragma unroll
+            for (int r = 0; r < 4; r++) h[r] = pack2(v[2 * r], v[2 * r + 1], type);
+            const auto lo = __builtin_amdgcn_permlane16_swap(h[0], h[2], false, false);
+            const auto hi = __builtin_amdgcn_permlane16_swap(h[1], h[3], false, false);
+            const int n = ncol + j * 16 + (g16 & 1) * 16 + (g16 >> 1) * 8;
+            if (orow < olim && n < P.cols) *(v4i*)(row + n * 2) = v4i{(int)lo[0], (int)hi[0], (int)lo[1], (int)hi[1]};
           }
         }
-        store4(P.out, P.out_type, orow * P.cols + n, v, have, P.vec);
+      });
+      continue;
+    }
+    // Rows that allow no 16-byte stores: 8 rows at a time go through this wave's own strip of LDS; a lane then holds eight
+    // consecutive columns of a row.  (The loop is not unrolled: code for all of it would not stay in the instruction cache.)
+    constexpr int LR = TN / 8, PASS = 64 / LR > 8 ? 1 : 8 * LR / 64;  // lanes per row; passes over 8 rows
+    constexpr int pitch = TN * 4 + 16;                               // (16 bytes between the rows move their banks apart)
+    const int crow = lane / LR, ccol = lane % LR * 8, n = w.col0 + wn * TN + ccol;
+    float bias[8] = {};
+    if (finish && P.bias) {
+      if (P.bias_lds) {
+        bias8(bias, bias_lds + (num & 3) * (BN * 4), P.bias_type, wn * TN + ccol, BN - 1);
+      } else {
+        bias8(bias, P.bias, P.bias_type, (long)w.g * P.cols + n, (long)w.g * P.cols + P.cols - 1);
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
       }
     }
+    char* const stage = lds + 2 * kBuf + wave * kStage;
+    const int have = P.cols - n;
+    for (int half = 0; half < 2 * FM; half++) {
+      const int orow = orow0 + half * 8;
+      if (orow >= olim) break;
+      for_each<FM>([&](auto I) {  // (the accumulators are registers: their indexes have to be constants)
+        constexpr int i = decltype(I)::value;
+        if (half >> 1 == i && (lane >> 3 & 1) == (half & 1)) {
+#pragma unroll
+          for (int j = 0; j < FN; j++) *(v4f*)(stage + (lane & 7) * pitch + (j * 16 + 4 * (lane >> 4)) * 4) = acc[i][j];
+          asm volatile("; rows %0" ::"n"(i * 16));  // (keeps the branches' ends apart: merged, they would index acc at run time)
+        }
+      });
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+      for (int c = 0; c < PASS; c++) {
+        const int row = crow + c * (64 / LR);
+        if (row < 8 && orow + row < olim && have > 0) {
+          const v4f lo = *(const v4f*)(stage + row * pitch + ccol * 4), hi = *(const v4f*)(stage + row * pitch + ccol * 4 + 16);
+          float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+#pragma unroll
+          for (int r = 0; r < 8; r++) v[r] += bias[r];
+          if (ACT && finish && P.act) gelu8(v);
+          store8(out, type, (first + orow + row) * P.cols + n, v, have, P.wide);
+        }
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
   }
+  // the loads behind the last step have written their zeros before the LDS is given back
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
 }  // namespace sm3x

@@ -16,12 +16,12 @@ int sm3_mx4_gemm(const sm3_expert_desc* d, void* workspace, size_t workspace_byt
   if (err != SM3_OK) return err;
   if (d->rows == 0) return SM3_OK;
   const Plan pl = make_plan(d, true);
+  if (!fits(pl)) return SM3_ERR_UNSUPPORTED;
   if (pl.part_bytes && (!workspace || workspace_bytes < pl.part_bytes || (uintptr_t)workspace % 16)) return SM3_ERR_WORKSPACE;
   const Params P = params_of(d, pl, true, workspace);
   hipStream_t st = (hipStream_t)stream;
-  const dim3 grid = grid_of(pl);
-  if (pl.bm == 32) tile_kernel<K_MX4, M_NT, 32, 128, 1, 4><<<grid, 256, 0, st>>>(P);
-  else tile_kernel<K_MX4, M_NT, 128, 128, 2, 2><<<grid, 256, 0, st>>>(P);
+  if (pl.bm == 32) tile_kernel<K_MX4, M_NT, 32, 128, 1, 4, 2><<<grid_of(pl, 3), 256, 0, st>>>(P);
+  else tile_kernel<K_MX4, M_NT, 128, 128, 2, 2, 2><<<grid_of(pl, 2), 256, 0, st>>>(P);
   const int rc = launch_status();
   return rc != SM3_OK ? rc : finish(P, pl, d, st);
 }

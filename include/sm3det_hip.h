@@ -675,10 +675,11 @@ int sm3_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, long rows, i
  *   mode SM3_GEMM_NN: out (rows, cols) = p (rows, red) . q[g] (red, cols)
  *   mode SM3_GEMM_TN: out[g] (rows_out, cols) = p (rows of g, rows_out)^T . q (rows of g, cols); bias_grad[g] (rows_out) = column
  *                     sums of p over the rows of g (may be NULL).  Experts without rows get zeros.
- * 16-bit: p, q of type `type` (F16 | BF16), 16-byte aligned, ldp / ldq elements between rows (multiples of 8; elements behind
- * the row's end up to the next multiple of 8 are read and must be ZERO along the reduction); NT / NN weights of expert g start
- * at q + g * cols * ldq (NN: g * red * ldq).  out contiguous, of type `out_type` (16-bit: equal to `type`).
- * MX4: NT only; p / q = codes, p_scales / q_scales, red = k (padded rows as above), ldp / ldq ignored.
+ * 16-bit: p, q of type `type` (F16 | BF16), ldp / ldq elements between rows (>= the row's length); NT / NN weights of expert g
+ * start at q + g * cols * ldq (NN: g * red * ldq).  Rows that do not start at 16-byte addresses or are no multiple of 8 long are
+ * copied into padded ones in the workspace first.  out contiguous, out_type = type.
+ * MX4: NT only; q = codes, q_scales.  p = codes with p_scales, or p_scales = NULL: rows of type `type` (F32 | F16 | BF16), ldp
+ * elements apart, quantised into the workspace first.  red = k (rows packed as above), ldq ignored.
  * act: 0 none, 1 GELU (erf; MX4 only).  bias (num_groups, cols) / bias_grad (num_groups, rows_out) of type bias_type. */
 typedef struct sm3_expert_desc {
   int32_t mode, type, out_type, bias_type, act, num_groups;
@@ -697,10 +698,6 @@ size_t sm3_expert_gemm_h16_workspace_bytes(const sm3_expert_desc* desc);
 int sm3_expert_gemm_h16(const sm3_expert_desc* desc, void* workspace, size_t workspace_bytes, sm3_stream_t stream);
 size_t sm3_mx4_gemm_workspace_bytes(const sm3_expert_desc* desc);
 int sm3_mx4_gemm(const sm3_expert_desc* desc, void* workspace, size_t workspace_bytes, sm3_stream_t stream);
-/* dst (rows, kp) = src (rows, k; ld elements apart) of a 16-bit type, columns k .. kp - 1 zero: rows that are not 16-byte
- * aligned or not a multiple of 8 long, made readable for sm3_expert_gemm_h16.  kp % 8 == 0, kp >= k, dst 16-byte aligned. */
-int sm3_pad_rows_h16(const void* src, long rows, int k, long ld, void* dst, int kp, sm3_stream_t stream);
-
 #ifdef __cplusplus
 }
 #endif

@@ -1,6 +1,7 @@
 """ctypes signatures + thin tensor-level callers for the backbone (MoE ConvNeXt) entry points of
 libsm3det_hip.so (declared in include/sm3det_hip.h)."""
 import ctypes
+import struct
 
 import torch
 
@@ -34,9 +35,13 @@ class ExpertDesc(ctypes.Structure):
                [(n, P) for n in ('p', 'q', 'p_scales', 'q_scales', 'offsets', 'bias', 'bias_grad', 'out')]
 
 
+EXPERT_DESC = struct.Struct('=10i3q8Q')  # the same fields in order: packing bytes costs a fifth of filling the structure
+assert EXPERT_DESC.size == ctypes.sizeof(ExpertDesc)
+
+
 def signatures():
     D = ctypes.POINTER(GemmDesc)
-    XD = ctypes.POINTER(ExpertDesc)
+    XD = P  # an ExpertDesc by reference, or its bytes (EXPERT_DESC.pack)
     LL = ctypes.c_long
     return {
         'sm3_gemm_f32_counter_slots': (I, []),
@@ -103,7 +108,6 @@ def signatures():
         'sm3_expert_gemm_h16': (I, [XD, P, S, P]),
         'sm3_mx4_gemm_workspace_bytes': (S, [XD]),
         'sm3_mx4_gemm': (I, [XD, P, S, P]),
-        'sm3_pad_rows_h16': (I, [P, LL, I, LL, P, I, P]),
     }
 
 

@@ -17,6 +17,9 @@ struct Plan {
   int ntiles, splits;  // NT / NN: slices of the reduction
   long unit_rows, units;  // TN: reduction rows per work unit
   size_t part_bytes, bsum_bytes;
+  // copies of the operands made first: padded rows (16-bit), packed rows (4-bit; codes, then scales)
+  size_t p_bytes, p_scale_bytes, q_bytes;
+  size_t total() const { return part_bytes + bsum_bytes + p_bytes + p_scale_bytes + q_bytes; }
 };
 
 // jobs are counted in 31 bits
@@ -31,23 +34,31 @@ inline int check_desc(const sm3_expert_desc* d, bool mx4) {
   if (d->mode == SM3_GEMM_TN ? d->rows_out < 1 || d->bias || d->act : d->bias_grad != nullptr) return SM3_ERR_INVALID_ARG;
   const bool reads = d->rows > 0;  // (a weight gradient over no rows writes zeros)
   if (!d->out || (reads && (!d->p || !d->q))) return SM3_ERR_INVALID_ARG;
-  if ((uintptr_t)d->p % 16 || (uintptr_t)d->q % 16) return SM3_ERR_INVALID_ARG;
-  // 32-bit offsets inside a tile: 256 rows of either operand
+  // 32-bit offsets inside a tile: up to 256 rows of either operand
   const long most = 1L << 22;
+  const long prow = d->mode == SM3_GEMM_TN ? d->rows_out : d->red, qrow = d->mode == SM3_GEMM_NT ? d->red : d->cols;
+  if (prow > most || qrow > most) return SM3_ERR_UNSUPPORTED;
   if (mx4) {
-    if (!d->p_scales || !d->q_scales || (uintptr_t)d->p_scales % 4 || (uintptr_t)d->q_scales % 4) return SM3_ERR_INVALID_ARG;
-    if (d->red > most) return SM3_ERR_UNSUPPORTED;
+    if (!d->q_scales || (uintptr_t)d->q % 16 || (uintptr_t)d->q_scales % 4) return SM3_ERR_INVALID_ARG;
+    if (d->p_scales) {
+      if ((uintptr_t)d->p % 16 || (uintptr_t)d->p_scales % 4) return SM3_ERR_INVALID_ARG;
+    } else if (d->type < 0 || d->type > SM3_DT_BF16 || d->ldp < d->red) {
+      return SM3_ERR_INVALID_ARG;
+    }
   } else {
     if (d->type != SM3_DT_F16 && d->type != SM3_DT_BF16) return SM3_ERR_INVALID_ARG;
     if (d->out_type != d->type || d->act) return SM3_ERR_INVALID_ARG;
-    const long prow = d->mode == SM3_GEMM_TN ? d->rows_out : d->red, qrow = d->mode == SM3_GEMM_NT ? d->red : d->cols;
-    if (d->ldp % 8 || d->ldq % 8 || d->ldp < (prow + 7) / 8 * 8 || d->ldq < (qrow + 7) / 8 * 8) return SM3_ERR_INVALID_ARG;
-    if (d->ldp > most || d->ldq > most) return SM3_ERR_UNSUPPORTED;
+    if (d->ldp < prow || d->ldq < qrow) return SM3_ERR_INVALID_ARG;
   }
   return SM3_OK;
 }
 
-inline Plan make_plan(const sm3_expert_desc* d, bool mx4) {
+// rows the tile kernel can read as they are
+inline bool readable(const void* p, long ld, long row) {
+  return (uintptr_t)p % 16 == 0 && ld % 8 == 0 && row % 8 == 0 && ld <= 1L << 22;
+}
+
+inline Plan plan_tiles(const sm3_expert_desc* d, bool mx4) {
   Plan p{};
   const bool grouped = d->offsets != nullptr;
   if (d->mode == SM3_GEMM_TN) {
@@ -93,6 +104,23 @@ inline Plan make_plan(const sm3_expert_desc* d, bool mx4) {
     }
   }
   p.per_xcd = (tiles * p.splits + kNumXCD - 1) / kNumXCD;
+  return p;
+}
+
+inline Plan make_plan(const sm3_expert_desc* d, bool mx4) {
+  Plan p = plan_tiles(d, mx4);
+  if (mx4) {
+    if (!d->p_scales) {
+      const size_t kp = ((size_t)d->red + 127) / 128 * 128;
+      p.p_bytes = align_up(d->rows * kp / 2, 256);
+      p.p_scale_bytes = align_up(d->rows * kp / 32, 256);
+    }
+  } else {
+    const long prow = d->mode == SM3_GEMM_TN ? d->rows_out : d->red, qrow = d->mode == SM3_GEMM_NT ? d->red : d->cols;
+    const long qrows = d->mode == SM3_GEMM_TN ? d->rows : (long)d->num_groups * (d->mode == SM3_GEMM_NT ? d->cols : d->red);
+    if (!readable(d->p, d->ldp, prow)) p.p_bytes = align_up((size_t)d->rows * ((prow + 7) / 8 * 8) * 2, 256);
+    if (!readable(d->q, d->ldq, qrow)) p.q_bytes = align_up((size_t)qrows * ((qrow + 7) / 8 * 8) * 2, 256);
+  }
   return p;
 }
 
@@ -190,10 +218,24 @@ static __global__ void __launch_bounds__(256) join_units_kernel(const float* __r
   store8(out, type, (long)g * n + i, v, have, whole && (uintptr_t)out % 16 == 0);
 }
 
-inline Params params_of(const sm3_expert_desc* d, const Plan& pl, bool mx4, void* ws) {
+// parts of the workspace
+struct Spaces {
+  char *p, *p_scales, *q;
+  float *part, *bsum;
+  Spaces(const Plan& pl, void* ws) {
+    char* at = (char*)ws;
+    p = at;
+    p_scales = (at += pl.p_bytes);
+    q = (at += pl.p_scale_bytes);
+    part = pl.part_bytes ? (float*)(at + pl.q_bytes) : nullptr;
+    bsum = pl.bsum_bytes ? (float*)(at + pl.q_bytes + pl.part_bytes) : nullptr;
+  }
+};
+
+inline Params params_of(const sm3_expert_desc* d, const Plan& pl, bool mx4, const Spaces& ws) {
   Params P{};
-  P.p = (const char*)d->p;
-  P.q = (const char*)d->q;
+  P.p = pl.p_bytes ? ws.p : (const char*)d->p;
+  P.q = pl.q_bytes ? ws.q : (const char*)d->q;
   P.S = d->rows;
   P.G = d->num_groups;
   P.offsets = d->offsets;
@@ -210,25 +252,26 @@ inline Params params_of(const sm3_expert_desc* d, const Plan& pl, bool mx4, void
     P.ldps = P.ldqs = kp / 32;
     P.strideq = d->cols * P.ldq;
     P.strideqs = d->cols * P.ldqs;
-    P.ps = d->p_scales;
+    P.ps = pl.p_scale_bytes ? (const unsigned char*)ws.p_scales : d->p_scales;
     P.qs = d->q_scales;
   } else {
-    P.ldp = d->ldp * 2;
-    P.ldq = d->ldq * 2;
+    const long prow = d->mode == SM3_GEMM_TN ? d->rows_out : d->red, qrow = d->mode == SM3_GEMM_NT ? d->red : d->cols;
+    P.ldp = pl.p_bytes ? (prow + 7) / 8 * 16 : d->ldp * 2;
+    P.ldq = pl.q_bytes ? (qrow + 7) / 8 * 16 : d->ldq * 2;
     P.red = d->red * 2L;
     P.qred = d->red;
     P.strideq = (d->mode == SM3_GEMM_NT ? (long)d->cols : (long)d->red) * P.ldq;
-    // 16-byte granules that straddle the end of the reduction hold zeros behind it (the caller's rows are padded)
+    // (rows whose length is no multiple of 8 are padded copies: the granule at the end of the reduction holds zeros)
     if (d->mode != SM3_GEMM_TN) P.red = (P.red + 15) & ~15L;
   }
   P.ntiles = pl.ntiles;
   P.splits = pl.splits;
   P.unit_rows = pl.unit_rows;
-  P.part = pl.part_bytes ? (float*)ws : nullptr;
+  P.part = ws.part;
   const long bes = d->bias_type == SM3_DT_F32 ? 4 : 2;
   P.bias_lds = d->bias && (uintptr_t)d->bias % 4 == 0 && d->cols * bes % 4 == 0;
   P.wide = P.part ? d->cols % 4 == 0 : d->cols % (d->out_type == SM3_DT_F32 ? 4 : 8) == 0 && (uintptr_t)d->out % 16 == 0;
-  P.bsum = pl.bsum_bytes ? (float*)((char*)ws + pl.part_bytes) : nullptr;
+  P.bsum = ws.bsum;
   return P;
 }
 

@@ -7,8 +7,7 @@ using namespace sm3x;
 extern "C" {
 
 size_t sm3_mx4_gemm_workspace_bytes(const sm3_expert_desc* d) {
-  if (check_desc(d, true) != SM3_OK) return 0;
-  return make_plan(d, true).part_bytes;
+  return check_desc(d, true) == SM3_OK ? make_plan(d, true).total() : 0;
 }
 
 int sm3_mx4_gemm(const sm3_expert_desc* d, void* workspace, size_t workspace_bytes, sm3_stream_t stream) {
@@ -17,9 +16,15 @@ int sm3_mx4_gemm(const sm3_expert_desc* d, void* workspace, size_t workspace_byt
   if (d->rows == 0) return SM3_OK;
   const Plan pl = make_plan(d, true);
   if (!fits(pl)) return SM3_ERR_UNSUPPORTED;
-  if (pl.part_bytes && (!workspace || workspace_bytes < pl.part_bytes || (uintptr_t)workspace % 16)) return SM3_ERR_WORKSPACE;
-  const Params P = params_of(d, pl, true, workspace);
+  const size_t need = pl.total();
+  if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16)) return SM3_ERR_WORKSPACE;
+  const Spaces ws(pl, workspace);
+  const Params P = params_of(d, pl, true, ws);
   hipStream_t st = (hipStream_t)stream;
+  if (pl.p_bytes) {
+    const int rc = sm3_mx4_quantize(d->p, d->type, d->rows, d->red, d->ldp, (uint8_t*)ws.p, (uint8_t*)ws.p_scales, stream);
+    if (rc != SM3_OK) return rc;
+  }
   if (pl.bm == 32) tile_kernel<K_MX4, M_NT, 32, 128, 1, 4, 2><<<grid_of(pl, 3), 256, 0, st>>>(P);
   else tile_kernel<K_MX4, M_NT, 128, 128, 2, 2, 2><<<grid_of(pl, 2), 256, 0, st>>>(P);
   const int rc = launch_status();

@@ -8,20 +8,19 @@ block of ``backbone_ops.moe_block``.  ``offsets`` are what ``sm3_moe_plan`` leav
 counts): the host never reads them, so calls are free of synchronisation and can be captured into a HIP graph.
 
 * types: x, w both bfloat16 or both float16, fp32 accumulation, results rounded once; b of x's type or float32.
-* any sizes (rows of a length that is no multiple of 8, or not 16-byte aligned, are copied into padded rows first).
+* any sizes and row strides (rows of a length that is no multiple of 8, or not 16-byte aligned, are copied into padded rows of
+  the workspace first).
 * rows of no expert (before ``offsets[0]``, behind ``offsets[-1]``): y and dx are zero there and they enter no gradient.
   Offsets outside [0, rows] are clamped, decreasing ones made monotone.
 * an expert without rows gets zero gradients (never an uninitialised one).
 * gradients do not depend on the order in which workgroups run: split reductions are added in a fixed order, no atomics.
 """
-import ctypes
-
 import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from . import _lib_backbone as LB
-from ._lib import SM3Error, check, lib, require_gpu, stream_ptr, workspace
+from ._lib import SM3Error, check, lib, require_gpu
 
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
@@ -35,83 +34,100 @@ def check_offsets(offsets, num_groups, device, name):
     return offsets.contiguous()
 
 
-def run_desc(fn, desc, device, flops, nbytes, what):
-    """enqueue one grouped product (sm3_<fn>) on the current stream of `device`, its workspace from torch's allocator"""
+_NEED = {}  # (entry point, sizes and types of a call) -> bytes of workspace: a query per new size, not per call
+
+
+def launch(fn, device, mode, dtype, out, p, q, rows, red, cols, *, rows_out=0, ldp=0, ldq=0, groups=1, offsets=None, bias=None,
+           bias_grad=None, act=0, p_scales=None, q_scales=None, aligned=0):
+    """enqueue one grouped product (sm3_<fn>) on torch's current stream of `device`, workspace from torch's allocator.
+    `aligned`: what decides, beside the sizes, whether operands are copied (the operands' addresses modulo 16)."""
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return launch(fn, device, mode, dtype, out, p, q, rows, red, cols, rows_out=rows_out, ldp=ldp, ldq=ldq, groups=groups,
+                          offsets=offsets, bias=bias, bias_grad=bias_grad, act=act, p_scales=p_scales, q_scales=q_scales,
+                          aligned=aligned)
     L = lib()
-    with torch.cuda.device(device):
-        need = getattr(L, f'sm3_{fn}_workspace_bytes')(ctypes.byref(desc))
-        ws = workspace(need, device) if need else None
-        with LB._Prof(what, flops, nbytes):
-            check(getattr(L, 'sm3_' + fn)(ctypes.byref(desc), None if ws is None else ws.data_ptr(), need, stream_ptr()),
-                  what)
-
-
-def readable_rows(t):
-    """`t` (..., K) as rows the kernels can read: unit stride along K, 16-byte aligned rows, zeros up to the next multiple of
-    8 -> (tensor, elements between rows).  A 2-D tensor may keep a row stride; everything else is made contiguous."""
-    K = t.shape[-1]
-    ld = t.stride(0) if t.dim() == 2 and t.shape[0] > 1 else K
-    if t.stride(-1) != 1 and K > 1 or (t.dim() == 2 and ld < K) or (t.dim() != 2 and not t.is_contiguous()):
-        t, ld = t.contiguous(), K
-    if K % 8 == 0 and ld % 8 == 0 and ld <= 1 << 22 and t.data_ptr() % 16 == 0:
-        return t, ld
-    kp = (K + 7) // 8 * 8
-    rows = t.numel() // K
-    out = torch.empty(*t.shape[:-1], kp, dtype=t.dtype, device=t.device)
-    with torch.cuda.device(t.device):
-        LB.call('pad_rows_h16', t, rows, K, ld, out, kp, nbytes=2.0 * rows * (K + kp))
-    return out, kp
-
-
-def _desc(mode, p, ldp, q, ldq, out, offsets, groups, rows, red, cols, rows_out=0, bias=None, bias_grad=None):
-    d = LB.ExpertDesc()
-    d.mode, d.type, d.out_type = mode, DTYPES[p.dtype], DTYPES[out.dtype]
     b = bias if bias is not None else bias_grad
-    d.bias_type = DTYPES[b.dtype] if b is not None else 0
-    d.num_groups, d.red, d.cols, d.rows_out = groups, red, cols, rows_out
-    d.rows, d.ldp, d.ldq = rows, ldp, ldq
-    d.p, d.q, d.out, d.offsets = LB._p(p), LB._p(q), LB._p(out), LB._p(offsets)
-    d.bias, d.bias_grad = LB._p(bias), LB._p(bias_grad)
-    return d
+    out_type = DTYPES[out.dtype]
+    desc = LB.EXPERT_DESC.pack(
+        mode, dtype, out_type, 0 if b is None else DTYPES[b.dtype], act, groups, red, cols, rows_out, 0, rows, ldp, ldq,
+        p.data_ptr(), q.data_ptr(), 0 if p_scales is None else p_scales.data_ptr(), 0 if q_scales is None else q_scales.data_ptr(),
+        0 if offsets is None else offsets.data_ptr(), 0 if bias is None else bias.data_ptr(),
+        0 if bias_grad is None else bias_grad.data_ptr(), out.data_ptr())
+    key = (fn, mode, dtype, out_type, groups, red, cols, rows_out, rows, ldp, ldq, offsets is None, bias_grad is None,
+           p_scales is None, aligned)
+    need = _NEED.get(key)
+    if need is None:
+        if len(_NEED) > 4096:
+            _NEED.clear()
+        need = _NEED[key] = getattr(L, f'sm3_{fn}_workspace_bytes')(desc)
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    args = (desc, None if ws is None else ws.data_ptr(), need, torch._C._cuda_getCurrentRawStream(device.index))
+    if LB.PROFILE is None:
+        code = getattr(L, 'sm3_' + fn)(*args)
+    else:
+        n = rows_out if mode == LB.TN else cols
+        with LB._Prof(f'{fn}_{("nt", "nn", "tn")[mode]}', 2.0 * rows * n * (cols if mode == LB.TN else red)):
+            code = getattr(L, 'sm3_' + fn)(*args)
+    if code:
+        check(code, fn)
+
+
+def rows_of(t):
+    """a 2-D tensor as rows with unit stride along them -> (tensor, elements between rows); copied only where it has none"""
+    n, k = t.shape
+    s0, s1 = t.stride()
+    if n <= 1:
+        return (t, k) if s1 == 1 or k == 1 else (t.contiguous(), k)
+    if (s1 == 1 or k == 1) and s0 >= k:
+        return t, s0
+    return t.contiguous(), k
+
+
+def _forward(x, w, offsets, b):
+    S, K = x.shape
+    E, N, _ = w.shape
+    y = torch.empty(S, N, dtype=x.dtype, device=x.device)
+    x, ldx = rows_of(x)
+    w = w.contiguous()
+    if S:
+        launch('expert_gemm_h16', x.device, LB.NT, DTYPES[x.dtype], y, x, w, S, K, N, ldp=ldx, ldq=K, groups=E, offsets=offsets,
+               bias=b, aligned=(x.data_ptr() | w.data_ptr()) & 15 and (x.data_ptr() & 15, w.data_ptr() & 15))
+    return y, x, w
 
 
 class _ExpertLinear(Function):
     @staticmethod
     def forward(ctx, x, w, offsets, b):
-        S, K = x.shape
-        E, N, _ = w.shape
-        y = torch.empty(S, N, dtype=x.dtype, device=x.device)
-        xr, ldx = readable_rows(x)
-        wr, ldw = readable_rows(w)
-        if S:
-            run_desc('expert_gemm_h16', _desc(LB.NT, xr, ldx, wr, ldw, y, offsets, E, S, K, N, bias=b), x.device,
-                     2.0 * S * N * K, 2.0 * (S * (N + K) + E * N * K), 'expert_linear')
-        ctx.save_for_backward(xr, wr, offsets)
-        ctx.meta = (S, K, E, N, ldx, ldw, None if b is None else b.dtype)
+        y, x, w = _forward(x, w, offsets, b)
+        ctx.save_for_backward(x, w, offsets)
+        ctx.b_dtype = None if b is None else b.dtype
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        xr, wr, offsets = ctx.saved_tensors
-        S, K, E, N, ldx, ldw, b_dtype = ctx.meta
-        dev = xr.device
-        dyr, lddy = readable_rows(dy)
-        flops, nbytes = 2.0 * S * N * K, 2.0 * (S * (N + K) + E * N * K)
+        x, w, offsets = ctx.saved_tensors
+        S, K = x.shape
+        E, N, _ = w.shape
+        dev, dt = x.device, DTYPES[x.dtype]
+        dy, lddy = rows_of(dy)
+        x, ldx = rows_of(x)
+        need = ctx.needs_input_grad
         dx = dw = db = None
-        if ctx.needs_input_grad[0]:
-            dx = torch.empty(S, K, dtype=xr.dtype, device=dev)
+        if need[0]:
+            dx = torch.empty(S, K, dtype=x.dtype, device=dev)
             if S:
-                run_desc('expert_gemm_h16', _desc(LB.NN, dyr, lddy, wr, ldw, dx, offsets, E, S, N, K), dev, flops, nbytes,
-                         'expert_linear_dgrad')
-        if ctx.needs_input_grad[1] or ctx.needs_input_grad[3]:
+                launch('expert_gemm_h16', dev, LB.NN, dt, dx, dy, w, S, N, K, ldp=lddy, ldq=K, groups=E, offsets=offsets,
+                       aligned=(dy.data_ptr() | w.data_ptr()) & 15 and (dy.data_ptr() & 15, w.data_ptr() & 15))
+        if need[1] or need[3]:
             # the bias gradient is a by-product of the weight gradient's pass over dy
-            dw = torch.empty(E, N, K, dtype=xr.dtype, device=dev)
-            if b_dtype is not None and ctx.needs_input_grad[3]:
-                db = torch.empty(E, N, dtype=b_dtype, device=dev)
-            run_desc('expert_gemm_h16', _desc(LB.TN, dyr, lddy, xr, ldx, dw, offsets, E, S, 1, K, rows_out=N, bias_grad=db),
-                     dev, flops, nbytes, 'expert_linear_wgrad')
-            if not ctx.needs_input_grad[1]:
+            dw = torch.empty(E, N, K, dtype=x.dtype, device=dev)
+            if need[3] and ctx.b_dtype is not None:
+                db = torch.empty(E, N, dtype=ctx.b_dtype, device=dev)
+            launch('expert_gemm_h16', dev, LB.TN, dt, dw, dy, x, S, 1, K, rows_out=N, ldp=lddy, ldq=ldx, groups=E, offsets=offsets,
+                   bias_grad=db, aligned=(dy.data_ptr() | x.data_ptr()) & 15 and (dy.data_ptr() & 15, x.data_ptr() & 15))
+            if not need[1]:
                 dw = None
         return dx, dw, None, db
 
@@ -132,4 +148,7 @@ def expert_linear(x, w, offsets, b=None):
             raise SM3Error(f'expert_linear: b must be {tuple(w.shape[:2])} of {x.dtype} or float32, got {tuple(b.shape)} of '
                            f'{b.dtype}')
         b = b.contiguous()
-    return _ExpertLinear.apply(x, w, check_offsets(offsets, w.shape[0], x.device, 'expert_linear'), b)
+    offsets = check_offsets(offsets, w.shape[0], x.device, 'expert_linear')
+    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or (b is not None and b.requires_grad)):
+        return _ExpertLinear.apply(x, w, offsets, b)
+    return _forward(x, w, offsets, b)[0]

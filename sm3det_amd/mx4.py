@@ -16,7 +16,7 @@ import torch
 
 from . import _lib_backbone as LB
 from ._lib import SM3Error, require_gpu
-from .expert_ops import DTYPES, check_offsets, run_desc
+from .expert_ops import DTYPES, check_offsets, launch, rows_of
 
 ACTS = {None: 0, 'gelu': 1}
 
@@ -119,15 +119,13 @@ def _product(what, x, w, offsets, b, act, out_dtype):
     y = torch.empty(M, N, dtype=out_dtype, device=w.device)
     if M == 0:
         return y
-    xq = x if packed else quantize(x)
-    d = LB.ExpertDesc()
-    d.mode, d.out_type, d.act, d.num_groups = LB.NT, DTYPES[out_dtype], ACTS[act], groups
-    d.bias_type = DTYPES[b.dtype] if b is not None else 0
-    d.red, d.cols, d.rows = w.k, N, M
-    d.p, d.q, d.out = LB._p(xq.codes), LB._p(w.codes), LB._p(y)
-    d.p_scales, d.q_scales, d.bias, d.offsets = LB._p(xq.scales), LB._p(w.scales), LB._p(b), LB._p(offsets)
-    run_desc('mx4_gemm', d, w.device, 2.0 * M * N * w.k, 0.53 * (M + groups * N) * w.k + y.element_size() * M * N,
-             what.replace('.', '_'))
+    if packed:
+        launch('mx4_gemm', w.device, LB.NT, 0, y, x.codes, w.codes, M, w.k, N, groups=groups, offsets=offsets, bias=b, act=ACTS[act],
+               p_scales=x.scales, q_scales=w.scales)
+    else:
+        x, ldx = rows_of(x)
+        launch('mx4_gemm', w.device, LB.NT, DTYPES[x.dtype], y, x, w.codes, M, w.k, N, ldp=ldx, groups=groups, offsets=offsets,
+               bias=b, act=ACTS[act], q_scales=w.scales)
     return y
 
 

@@ -600,7 +600,7 @@ class _MoEBlock(Function):
 
     @staticmethod
     def forward(ctx, x, w49, bdw, lnw, lnb, wp, bp, wn, sim, temp, w1, b1, w2, b2, gamma, rs, noise, eps, B, H, W, k,
-                train, clamp_max, loss_coef, forced_topk=None):
+                train, clamp_max, loss_coef, forced_topk=None, experts=None):
         from . import _lib
         x = _chk(x, 'x')
         T, C = x.shape
@@ -657,6 +657,13 @@ class _MoEBlock(Function):
                  nbytes=4.0 * S * C)
         else:
             call('moe_dispatch', xn, slot_token, xslot, S, C, nbytes=8.0 * S * C)
+        if experts is not None:  # (inference only: moe_block refuses it where a gradient would be needed)
+            yslot = experts(xslot, offsets)
+            out = _e(T, C, like=x)
+            call('moe_combine_fwd', yslot, token_slot, gates, x, gamma, rs, H * W, out, T, C, k,
+                 nbytes=4.0 * (k + 2) * T * C)
+            ctx.mark_non_differentiable(tot, offsets, top_idx)
+            return out, loss.reshape(()), tot, offsets, top_idx
         # experts: grouped GEMM pair over the expert-major slots
         hpre, act = _e(S, Hd, like=x, dtype=xn.dtype), _e(S, Hd, like=x, dtype=xn.dtype)
         ctx.wparams = (w1, w2)  # the parameters themselves (their data-parallel bucket slices receive the gradients)
@@ -765,12 +772,17 @@ class _MoEBlock(Function):
         _join_side(dev)
         return (dx, dw49, dbdw, dlnw, dlnb, dwp, dbp, dwn, dsim, None if dtemp is None else dtemp.reshape(temp.shape),
                 dw1, db1, dw2, db2, dgamma,
-                None, None, None, None, None, None, None, None, None, None, None)
+                None, None, None, None, None, None, None, None, None, None, None, None)
 
 
 def moe_block(x, w49, bdw, lnw, lnb, wp, bp, wn, sim, temp, w1, b1, w2, b2, gamma, rs, noise, eps, B, H, W, k, train,
-              clamp_max, loss_coef=1e-2, forced_topk=None):
+              clamp_max, loss_coef=1e-2, forced_topk=None, experts=None):
     """Returns (out (T,C), aux loss (scalar), [importance | load] (2E, non-differentiable), expert slot offsets
-    (E+1, int32, non-differentiable), top-(k+1) expert indices per token (T, min(k+1,E), int32, non-differentiable))."""
+    (E+1, int32, non-differentiable), top-(k+1) expert indices per token (T, min(k+1,E), int32, non-differentiable)).
+    experts: None, or a function (xslot (S,C), offsets) -> yslot (S,C) float32 that takes the place of the expert FFNs
+    (mx4.quantize_experts); inference only."""
+    if experts is not None and torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (x, w49, bdw, lnw, lnb, wp, bp, wn, sim, temp, w1, b1, w2, b2, gamma)):
+        raise SM3Error('quantised experts are for inference: run the module under torch.no_grad()')
     return _MoEBlock.apply(x, w49, bdw, lnw, lnb, wp, bp, wn, sim, temp, w1, b1, w2, b2, gamma, rs, noise, eps, B, H,
-                           W, k, train, clamp_max, loss_coef, forced_topk)
+                           W, k, train, clamp_max, loss_coef, forced_topk, experts)

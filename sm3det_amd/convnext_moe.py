@@ -138,6 +138,24 @@ class MoE_layer(nn.Module):
         self.last_expert_offsets = None  # device int32 (E+1): expert loads of the last forward (no sync)
         self.last_importance_load = None  # device fp32 (2E): [importance | load] of the last forward
         self.last_top_idx = None  # device int32 (T, min(k+1,E)): the routing of the last forward, best first
+        self._mx4 = None  # packed 4-bit (w1, w2) of mx4.quantize_experts; gone when the weights may change or move
+
+    def experts(self):
+        """what takes the place of the expert FFNs in this forward: None, or the 4-bit experts (evaluation only)"""
+        if self._mx4 is None:
+            return None
+        from . import mx4
+        (w1, w2), b1, b2 = self._mx4, self.b1, self.b2
+        return lambda xslot, offsets: mx4.expert_ffn(xslot, w1, b1.detach(), w2, b2.detach(), offsets)
+
+    def train(self, mode=True):
+        if mode:
+            self._mx4 = None
+        return super().train(mode)
+
+    def _apply(self, *args, **kwargs):
+        self._mx4 = None
+        return super()._apply(*args, **kwargs)
 
     # ---- reference key schema <-> fused storage ---------------------------------------------------------
     _FUSED = {'w1': 'pointwise_conv1.weight', 'b1': 'pointwise_conv1.bias',
@@ -152,6 +170,7 @@ class MoE_layer(nn.Module):
 
     def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys,
                               error_msgs):
+        self._mx4 = None
         for fused, ref in self._FUSED.items():
             keys = [f'{prefix}experts.{e}.{ref}' for e in range(self.num_experts)]
             if prefix + fused not in state_dict and all(k in state_dict for k in keys):
@@ -276,7 +295,7 @@ class ConvNeXtBlock(nn.Module):
         out, loss, tot, offsets, top_idx = ops.moe_block(
             x, w49, self.depthwise_conv.bias, self.norm.weight, self.norm.bias, *gate_args, moe.w1, moe.b1, moe.w2,
             moe.b2, self.gamma, rs, noise if train else None, self.norm.eps, B, H, W, moe.k, train, clamp_max,
-            moe.loss_coef, forced_topk)  # aux loss (:234-238) comes out of the block: coef * (cv^2(importance) + cv^2(load))
+            moe.loss_coef, forced_topk, moe.experts())  # aux loss (:234-238) comes out of the block: coef * (cv^2(importance) + cv^2(load))
         moe.last_expert_offsets = offsets
         moe.last_importance_load = tot
         moe.last_top_idx = top_idx

@@ -29,6 +29,7 @@ inline int check_desc(const sm3_expert_desc* d, bool mx4) {
   if (!d || d->num_groups < 1 || d->rows < 0 || d->rows > 0x7fffff00L || d->red < 1 || d->cols < 1) return SM3_ERR_INVALID_ARG;
   if (d->mode < SM3_GEMM_NT || d->mode > SM3_GEMM_TN || (mx4 && d->mode != SM3_GEMM_NT)) return SM3_ERR_INVALID_ARG;
   if (!d->offsets && d->num_groups != 1) return SM3_ERR_INVALID_ARG;
+  if (d->num_groups > 65535) return SM3_ERR_UNSUPPORTED;  // (a dimension of a grid)
   if (d->act < 0 || d->act > 1 || d->bias_type < 0 || d->bias_type > SM3_DT_BF16) return SM3_ERR_INVALID_ARG;
   if (d->out_type < 0 || d->out_type > SM3_DT_BF16) return SM3_ERR_INVALID_ARG;
   if (d->mode == SM3_GEMM_TN ? d->rows_out < 1 || d->bias || d->act : d->bias_grad != nullptr) return SM3_ERR_INVALID_ARG;
@@ -80,7 +81,6 @@ inline Plan plan_tiles(const sm3_expert_desc* d, bool mx4) {
         if (d->bias_grad) p.bsum_bytes = align_up((size_t)p.units * d->rows_out * 4, 256);
       }
     }
-    if (!p.part_bytes && d->bias_grad) p.bsum_bytes = align_up((size_t)p.units * d->rows_out * 4, 256);
     p.mtiles = p.units * mt;
     p.splits = 1;
     p.per_xcd = p.units * ((tiles + kNumXCD - 1) / kNumXCD);
@@ -158,9 +158,18 @@ static __global__ void __launch_bounds__(256) join_rows_kernel(const Params P) {
   }
 }
 
-// out[g][i] = sum over the work units of expert g, in their order; `n` values per unit
-static __global__ void __launch_bounds__(256) join_units_kernel(const float* __restrict__ part, const Params P, void* out,
-                                                                int type, long n) {
+// out[g][i] = sum over the work units of expert g, in their order; `n` values per unit.  Blocks [0, split) of a row of the grid
+// join the weight gradient's partials, the others the bias gradient's.
+struct Join {
+  const float* part;
+  void* out;
+  int type;
+  long n;
+};
+static __global__ void __launch_bounds__(256) join_units_kernel(const Params P, const Join a, const Join b, unsigned split) {
+  const Join J = blockIdx.x < split ? a : b;
+  const float* const part = J.part;
+  const long n = J.n;
   const int g = blockIdx.y, lane = threadIdx.x & 63;
   long first = 0;
   int count = 0;
@@ -196,7 +205,7 @@ static __global__ void __launch_bounds__(256) join_units_kernel(const float* __r
       }
     }
   }
-  const long i = ((long)blockIdx.x * 256 + threadIdx.x) * 8;
+  const long i = ((long)(blockIdx.x < split ? blockIdx.x : blockIdx.x - split) * 256 + threadIdx.x) * 8;
   if (i >= n) return;
   const int have = (int)(n - i < 8 ? n - i : 8);
   float v[8] = {};
@@ -215,7 +224,7 @@ static __global__ void __launch_bounds__(256) join_units_kernel(const float* __r
       for (int r = 0; r < 8; r++) v[r] += r < have ? at[r] : 0.f;
     }
   }
-  store8(out, type, (long)g * n + i, v, have, whole && (uintptr_t)out % 16 == 0);
+  store8(J.out, J.type, (long)g * n + i, v, have, whole && (uintptr_t)J.out % 16 == 0);
 }
 
 // parts of the workspace
@@ -272,6 +281,7 @@ inline Params params_of(const sm3_expert_desc* d, const Plan& pl, bool mx4, cons
   P.bias_lds = d->bias && (uintptr_t)d->bias % 4 == 0 && d->cols * bes % 4 == 0;
   P.wide = P.part ? d->cols % 4 == 0 : d->cols % (d->out_type == SM3_DT_F32 ? 4 : 8) == 0 && (uintptr_t)d->out % 16 == 0;
   P.bsum = ws.bsum;
+  P.db = d->bias_grad;
   return P;
 }
 
@@ -284,12 +294,11 @@ inline dim3 grid_of(const Plan& pl, int per_cu) {
 
 inline int finish(const Params& P, const Plan& pl, const sm3_expert_desc* d, hipStream_t st) {
   if (d->mode == SM3_GEMM_TN) {
+    if (!P.part) return SM3_OK;
     const long n = (long)P.rows_out * P.cols;
-    if (P.part)
-      join_units_kernel<<<dim3((unsigned)((n + 2047) / 2048), P.G), 256, 0, st>>>(P.part, P, P.out, P.out_type, n);
-    if (P.bsum)
-      join_units_kernel<<<dim3((unsigned)((P.rows_out + 2047) / 2048), P.G), 256, 0, st>>>(P.bsum, P, d->bias_grad, d->bias_type,
-                                                                                         P.rows_out);
+    const Join w = {P.part, P.out, P.out_type, n}, b = {P.bsum, d->bias_grad, d->bias_type, P.rows_out};
+    const unsigned nw = (unsigned)((n + 2047) / 2048), nb = P.bsum ? (unsigned)((P.rows_out + 2047) / 2048) : 0;
+    join_units_kernel<<<dim3(nw + nb, P.G), 256, 0, st>>>(P, w, b, nw);
   } else if (P.part) {
     join_rows_kernel<<<dim3((unsigned)((P.cols + 2047) / 2048), (unsigned)(P.S < 32768 ? P.S : 32768)), 256, 0, st>>>(P);
   }

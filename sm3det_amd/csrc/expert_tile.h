@@ -53,7 +53,8 @@ struct Params {
   int wide;                       // result rows allow 16-byte stores
   int bias_lds;                   // bias rows may be loaded as 4-byte words
   const void* bias;               // (G, cols) or null
-  float* bsum;                    // TN: per work unit column sums of p (units, rows_out) fp32, or null
+  void* db;                       // TN: column sums of p per expert (G, rows_out) of bias_type, or null;
+  float* bsum;                    // where units are parts of experts: per unit (units, rows_out) fp32
   const int* offsets;             // (G + 1) device, or null: one group of all S rows
   int G;
   long S;
@@ -702,7 +703,7 @@ __global__ void __launch_bounds__(WM * WN * 64, MINW) tile_kernel(const Params P
 #pragma unroll
       for (int j = 0; j < FN; j++) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
     if constexpr (MODE == M_TN) {
-      sums = P.bsum != nullptr && w.col0 == 0 && wn == 0;
+      sums = P.db != nullptr && w.col0 == 0 && wn == 0;
 #pragma unroll
       for (int i = 0; i < FM; i++) bacc[i] = 0.f;
     }
@@ -738,7 +739,11 @@ __global__ void __launch_bounds__(WM * WN * 64, MINW) tile_kernel(const Params P
         v += __shfl_xor(v, 16);
         v += __shfl_xor(v, 32);
         const int orow = w.prow0 + wm * TM + i * 16 + lane;
-        if (lane < 16 && orow < P.rows_out) P.bsum[(long)w.unit * P.rows_out + orow] = v;
+        if (lane < 16 && orow < P.rows_out) {
+          if (P.bsum) P.bsum[(long)w.unit * P.rows_out + orow] = v;
+          else if (P.bias_type == DT_F32) ((float*)P.db)[(long)w.g * P.rows_out + orow] = v;
+          else ((unsigned short*)P.db)[(long)w.g * P.rows_out + orow] = (unsigned short)pack2(v, 0.f, P.bias_type);
+        }
       }
     }
     void* const out = P.part ? (void*)P.part : P.out;

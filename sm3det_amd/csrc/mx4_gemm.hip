@@ -1,19 +1,36 @@
 // mx4_gemm.hip -- products of microscaled 4-bit rows, dense and grouped by expert: v_mfma_scale_f32_16x16x128_f8f6f4 with both
 // operands e2m1 and the blocks' scale bytes as its scale operands (no dequantised copy exists anywhere).
 #include "expert_plan.h"
+#include "mx4_few.h"
 
 using namespace sm3x;
+
+namespace {
+
+// A handful of rows per expert, not yet quantised: one launch without a workspace (mx4_few.hip).  Up to 16 rows an expert's
+// rows are one tile there; with more the weights would be read again for every 16 rows.
+bool few(const sm3_expert_desc* d) {
+  const long experts = d->num_groups < d->rows ? d->num_groups : d->rows;
+  return !d->p_scales && d->rows <= 16 * experts && row_tiles(d->rows, d->num_groups, d->offsets != nullptr, 16) < 65536;
+}
+
+}  // namespace
 
 extern "C" {
 
 size_t sm3_mx4_gemm_workspace_bytes(const sm3_expert_desc* d) {
-  return check_desc(d, true) == SM3_OK ? make_plan(d, true).total() : 0;
+  return check_desc(d, true) == SM3_OK && !few(d) ? make_plan(d, true).total() : 0;
 }
 
 int sm3_mx4_gemm(const sm3_expert_desc* d, void* workspace, size_t workspace_bytes, sm3_stream_t stream) {
   const int err = check_desc(d, true);
   if (err != SM3_OK) return err;
   if (d->rows == 0) return SM3_OK;
+  if (few(d)) {
+    const Few f = {d->p, d->ldp, (const unsigned char*)d->q, d->q_scales, d->red, (d->red + 127) / 128 * 128, d->cols,
+                   d->num_groups, (int)d->rows, d->offsets, d->bias, d->bias_type, d->act, d->out_type, d->out};
+    return launch_few(f, d->type, row_tiles(d->rows, d->num_groups, d->offsets != nullptr, 16), (hipStream_t)stream);
+  }
   const Plan pl = make_plan(d, true);
   if (!fits(pl)) return SM3_ERR_UNSUPPORTED;
   const size_t need = pl.total();

@@ -41,7 +41,7 @@ def launch(fn, device, mode, dtype, out, p, q, rows, red, cols, *, rows_out=0, l
            bias_grad=None, act=0, p_scales=None, q_scales=None, aligned=0):
     """enqueue one grouped product (sm3_<fn>) on torch's current stream of `device`, workspace from torch's allocator.
     `aligned`: what decides, beside the sizes, whether operands are copied (the operands' addresses modulo 16)."""
-    if device.index != torch.cuda.current_device():
+    if device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
             return launch(fn, device, mode, dtype, out, p, q, rows, red, cols, rows_out=rows_out, ldp=ldp, ldq=ldq, groups=groups,
                           offsets=offsets, bias=bias, bias_grad=bias_grad, act=act, p_scales=p_scales, q_scales=q_scales,

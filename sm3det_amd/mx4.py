@@ -15,7 +15,7 @@ experts of a backbone's MoE blocks (mmrotate/models/backbones/convnext_moe.py:22
 import torch
 
 from . import _lib_backbone as LB
-from ._lib import SM3Error, require_gpu
+from ._lib import SM3Error, check, lib, require_gpu
 from .expert_ops import DTYPES, check_offsets, launch, rows_of
 
 ACTS = {None: 0, 'gelu': 1}
@@ -32,17 +32,24 @@ class Mx4Tensor:
 
     def __init__(self, codes, scales, k):
         k = int(k)
+        cs, ss = codes.shape, scales.shape
+        kp = padded(k) if k > 0 else 0
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.device != scales.device:
             raise SM3Error('Mx4Tensor: codes and scales must be uint8 tensors on one device')
-        if k < 1 or codes.dim() < 2 or codes.shape[:-1] != scales.shape[:-1] or codes.shape[-1] * 2 != padded(k) or \
-                scales.shape[-1] * 32 != padded(k):
-            raise SM3Error(f'Mx4Tensor: rows of {k} elements need codes (..., {padded(max(k, 1)) // 2}) and scales '
-                           f'(..., {padded(max(k, 1)) // 32}), got {tuple(codes.shape)} and {tuple(scales.shape)}')
+        if kp == 0 or len(cs) < 2 or cs[:-1] != ss[:-1] or cs[-1] * 2 != kp or ss[-1] * 32 != kp:
+            raise SM3Error(f'Mx4Tensor: rows of {k} elements need codes (..., {kp // 2}) and scales (..., {kp // 32}), got '
+                           f'{tuple(cs)} and {tuple(ss)}')
         codes, scales = codes.contiguous(), scales.contiguous()
         # the kernels read 16-byte granules of codes and 4-byte words of scales
         self.codes = codes if codes.data_ptr() % 16 == 0 else codes.clone()
         self.scales = scales if scales.data_ptr() % 4 == 0 else scales.clone()
         self.k = k
+
+    @classmethod
+    def _of(cls, codes, scales, k):  # storage this module allocated itself
+        q = cls.__new__(cls)
+        q.codes, q.scales, q.k = codes, scales, k
+        return q
 
     @property
     def shape(self):
@@ -60,12 +67,28 @@ class Mx4Tensor:
         if dtype not in DTYPES:
             raise SM3Error(f'dequantize: float32, float16 or bfloat16, not {dtype}')
         require_gpu(self.codes)
-        y = torch.empty(self.shape, dtype=dtype, device=self.device)
-        rows = self.scales.numel() // self.scales.shape[-1]
-        with torch.cuda.device(self.device):
-            LB.call('mx4_dequantize', self.codes, self.scales, rows, self.k, y, DTYPES[dtype],
-                    nbytes=y.numel() * (y.element_size() + 0.53))
+        y = torch.empty(self.shape, dtype=dtype, device=self.codes.device)
+        rows = y.numel() // self.k
+        if rows:
+            _call('mx4_dequantize', self.codes.device, y.numel() * (y.element_size() + 0.53), self.codes.data_ptr(),
+                  self.scales.data_ptr(), rows, self.k, y.data_ptr(), DTYPES[dtype])
         return y
+
+
+def _call(name, device, nbytes, *args):
+    """sm3_<name>(*args, current stream of `device`)"""
+    if device.index != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            return _call(name, device, nbytes, *args)
+    fn = getattr(lib(), 'sm3_' + name)
+    stream = torch._C._cuda_getCurrentRawStream(device.index)
+    if LB.PROFILE is None:
+        code = fn(*args, stream)
+    else:
+        with LB._Prof(name, 0.0, nbytes):
+            code = fn(*args, stream)
+    if code:
+        check(code, name)
 
 
 def _no_grad(what, *tensors):
@@ -80,16 +103,15 @@ def quantize(x):
     if x.dtype not in DTYPES or x.dim() < 2 or x.shape[-1] < 1:
         raise SM3Error(f'mx4.quantize: (..., K) float32, float16 or bfloat16 rows expected, got {tuple(x.shape)} of {x.dtype}')
     K = x.shape[-1]
-    if not (x.dim() == 2 and x.shape[0] > 1 and x.stride(1) == 1 and x.stride(0) >= K):
-        x = x.contiguous()
-    ld = x.stride(0) if x.dim() == 2 and x.shape[0] > 1 else K
-    kp = padded(K)
+    x, ld = rows_of(x) if x.dim() == 2 else (x.contiguous(), K)
+    kp = (K + 127) // 128 * 128
     codes = torch.empty(*x.shape[:-1], kp // 2, dtype=torch.uint8, device=x.device)
     scales = torch.empty(*x.shape[:-1], kp // 32, dtype=torch.uint8, device=x.device)
-    with torch.cuda.device(x.device):
-        LB.call('mx4_quantize', x, DTYPES[x.dtype], x.numel() // K, K, ld, codes, scales,
-                nbytes=x.numel() * (x.element_size() + 0.53))
-    return Mx4Tensor(codes, scales, K)
+    n = x.numel()
+    if n:
+        _call('mx4_quantize', x.device, n * (x.element_size() + 0.53), x.data_ptr(), DTYPES[x.dtype], n // K, K, ld, codes.data_ptr(),
+              scales.data_ptr())
+    return Mx4Tensor._of(codes, scales, K)
 
 
 def _product(what, x, w, offsets, b, act, out_dtype):
@@ -98,51 +120,86 @@ def _product(what, x, w, offsets, b, act, out_dtype):
     if act not in ACTS:
         raise SM3Error(f"{what}: act must be None or 'gelu', not {act!r}")
     packed = isinstance(x, Mx4Tensor)
-    require_gpu(w.codes, x.codes if packed else x, offsets, b)
-    if len(x.shape) != 2 or x.shape[1] != w.k:
-        raise SM3Error(f'{what}: x {tuple(x.shape)} does not match w {tuple(w.shape)}')
+    codes, device = w.codes, w.codes.device
+    lead, k = codes.shape[:-1], w.k
+    if len(lead) != (1 if offsets is None else 2):
+        raise SM3Error(f"{what}: w must be {'(N, K)' if offsets is None else '(E, N, K)'}, got {tuple(w.shape)}")
+    require_gpu(codes, x.codes if packed else x, b)
+    if packed:
+        if x.codes.dim() != 2 or x.k != k:
+            raise SM3Error(f'{what}: x {tuple(x.shape)} does not match w {tuple(w.shape)}')
+    elif x.dim() != 2 or x.shape[1] != k or x.dtype not in DTYPES:
+        raise SM3Error(f'{what}: x (M, {k}) of float32, float16 or bfloat16 expected, got {tuple(x.shape)} of {x.dtype}')
     if out_dtype is None:
         out_dtype = torch.float32 if packed else x.dtype
-    if out_dtype not in DTYPES:
+    elif out_dtype not in DTYPES:
         raise SM3Error(f'{what}: float32, float16 or bfloat16 results, not {out_dtype}')
-    groups, N = (1, w.shape[0]) if offsets is None else w.shape[:2]
+    groups, N = lead if offsets is not None else (1, lead[0])
     if N < 1 or groups < 1:
         raise SM3Error(f'{what}: w {tuple(w.shape)} has no rows')
-    if x.device != w.device or (b is not None and b.device != w.device):
+    if x.device != device or (b is not None and b.device != device):
         raise SM3Error(f'{what}: x, w and b must be on one device')
     if b is not None:
-        if b.shape != w.shape[:-1] or b.dtype not in DTYPES:
-            raise SM3Error(f'{what}: b must be {tuple(w.shape[:-1])} of a floating type, got {tuple(b.shape)} of {b.dtype}')
+        if b.shape != lead or b.dtype not in DTYPES:
+            raise SM3Error(f'{what}: b must be {tuple(lead)} of a floating type, got {tuple(b.shape)} of {b.dtype}')
         b = b.contiguous()
-    _no_grad(what, None if packed else x, b)
-    M = x.shape[0]
-    y = torch.empty(M, N, dtype=out_dtype, device=w.device)
+    if torch.is_grad_enabled():
+        _no_grad(what, None if packed else x, b)
+    if offsets is not None:
+        offsets = check_offsets(offsets, groups, device, what)
+    M = x.codes.shape[0] if packed else x.shape[0]
+    y = torch.empty(M, N, dtype=out_dtype, device=device)
     if M == 0:
         return y
     if packed:
-        launch('mx4_gemm', w.device, LB.NT, 0, y, x.codes, w.codes, M, w.k, N, groups=groups, offsets=offsets, bias=b, act=ACTS[act],
+        launch('mx4_gemm', device, LB.NT, 0, y, x.codes, codes, M, k, N, groups=groups, offsets=offsets, bias=b, act=ACTS[act],
                p_scales=x.scales, q_scales=w.scales)
     else:
         x, ldx = rows_of(x)
-        launch('mx4_gemm', w.device, LB.NT, DTYPES[x.dtype], y, x, w.codes, M, w.k, N, ldp=ldx, groups=groups, offsets=offsets,
-               bias=b, act=ACTS[act], q_scales=w.scales)
+        launch('mx4_gemm', device, LB.NT, DTYPES[x.dtype], y, x, codes, M, k, N, ldp=ldx, groups=groups, offsets=offsets, bias=b,
+               act=ACTS[act], q_scales=w.scales)
     return y
 
 
 def linear(x, w, b=None, act=None, out_dtype=None):
     """act(Q(x) . w^T + b): x (M, K) of a floating type (quantised in the call) or an Mx4Tensor, w an Mx4Tensor (N, K), b (N)
     or None, act None or 'gelu' (erf).  The result has x's type, or out_dtype (float32 where x is packed)."""
-    if isinstance(w, Mx4Tensor) and len(w.shape) != 2:
-        raise SM3Error(f'mx4.linear: w must be (N, K), got {tuple(w.shape)}')
     return _product('mx4.linear', x, w, None, b, act, out_dtype)
 
 
 def expert_linear(x, w, offsets, b=None, act=None, out_dtype=None):
     """`linear` with one weight per expert: w an Mx4Tensor (E, N, K), b (E, N) or None, rows [offsets[g], offsets[g + 1]) of x
     belong to expert g (offsets (E + 1) int32 on the device, never read by the host); rows of no expert give zeros."""
-    if isinstance(w, Mx4Tensor):
-        if len(w.shape) != 3:
-            raise SM3Error(f'mx4.expert_linear: w must be (E, N, K), got {tuple(w.shape)}')
-        require_gpu(w.codes, offsets)
-        offsets = check_offsets(offsets, w.shape[0], w.device, 'mx4.expert_linear')
+    if offsets is None:
+        raise SM3Error('mx4.expert_linear: offsets (E + 1) are missing')
     return _product('mx4.expert_linear', x, w, offsets, b, act, out_dtype)
+
+
+def expert_ffn(x, w1, b1, w2, b2, offsets):
+    """Linear -> GELU -> Linear of each row's expert (FFN.forward, convnext_moe.py:397-405) on 4-bit operands: x (S, C),
+    w1 (E, 4C, C) and w2 (E, C, 4C) packed, -> (S, C) float32.  The hidden rows live as bfloat16 between the two products (their
+    8 bits go through a second rounding to e2m1's 2; bfloat16 keeps fp32's range)."""
+    h = expert_linear(x, w1, offsets, b1, act='gelu', out_dtype=torch.bfloat16)
+    return expert_linear(h, w2, offsets, b2, out_dtype=torch.float32)
+
+
+def quantize_experts(module):
+    """Pack the experts of every MoE layer inside `module` (a backbone or a detector in evaluation mode): its forward under
+    ``torch.no_grad()`` then runs them on the 4-bit products -- router, combine, dense blocks and everything else as before.
+    The packed weights are a snapshot: ``train()``, ``load_state_dict()`` and moving the module drop them.  -> layers packed."""
+    from .convnext_moe import MoE_layer
+    layers = [m for m in module.modules() if isinstance(m, MoE_layer)]
+    for m in layers:
+        if m.training:
+            raise SM3Error('mx4.quantize_experts: call module.eval() first (4-bit experts are for inference)')
+    for m in layers:
+        m._mx4 = (quantize(m.w1.detach()), quantize(m.w2.detach()))
+    return len(layers)
+
+
+def restore_experts(module):
+    """undo `quantize_experts`"""
+    from .convnext_moe import MoE_layer
+    for m in module.modules():
+        if isinstance(m, MoE_layer):
+            m._mx4 = None

@@ -83,7 +83,7 @@ def test_the_abi_refuses_types_strides_and_small_workspaces(L):
         assert L.sm3_mx4_gemm(ctypes.byref(_desc(**kw)), None, 0, None) == -1, kw
     # operands that have to be copied need room: unaligned or odd 16-bit rows, floating rows of a 4-bit product
     for fn, kw in (('sm3_expert_gemm_h16', dict(p=(1 << 20) + 2)), ('sm3_expert_gemm_h16', dict(red=63)),
-                   ('sm3_expert_gemm_h16', dict(ldp=68)), ('sm3_mx4_gemm', dict(p_scales=None))):
+                   ('sm3_expert_gemm_h16', dict(ldp=68)), ('sm3_mx4_gemm', dict(p_scales=None, rows=400))):
         d = _desc(**kw)
         assert getattr(L, fn + '_workspace_bytes')(ctypes.byref(d)) > 0, kw
         assert getattr(L, fn)(ctypes.byref(d), None, 0, None) == -2, kw

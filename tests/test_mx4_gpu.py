@@ -122,7 +122,7 @@ def _check(y, h, mag, k, act, dtype, what=''):
 
 
 LINEAR = [(1, 1, 1), (1, 8, 32), (2, 130, 96), (17, 64, 128), (32, 257, 300), (33, 40, 256), (129, 128, 512), (200, 250, 603),
-          (1, 4096, 1024), (5, 96, 4096), (300, 384, 96), (700, 130, 2000)]
+          (1, 4096, 1024), (5, 96, 4096), (300, 384, 96), (700, 130, 2000), (16, 17, 129), (15, 33, 1000), (3, 250, 603)]
 
 
 @pytest.mark.parametrize('dtype', DT)
@@ -244,3 +244,93 @@ def test_the_same_call_gives_the_same_bits():
     x, w = _rows(1, 6, 4000, torch.float32), mx4.quantize(_rows(2, 100, 4000, torch.float32))
     first = mx4.linear(x, w)
     assert all(torch.equal(mx4.linear(x, w), first) for _ in range(5))
+
+
+# ---- the operators together: quantise, first product with GELU, second product, by expert -- and the backbone's MoE blocks
+def _plain_ffn(x, w1, b1, w2, b2, offsets):
+    """64-bit restatement of expert_ffn on the packed weights' values -> (y, sums of magnitudes, largest hidden value)"""
+    e, c = w1.shape[0], x.shape[1]
+    rows = x.shape[0]
+    y = torch.zeros(rows, c, dtype=torch.float64, device='cuda')
+    mag, top = torch.zeros_like(y), 0.0
+    for g, (p, q) in enumerate(spans(offsets, rows)):
+        if p == q:
+            continue
+        xv = torch.from_numpy(quantize_ref(x[p:q].double().cpu().numpy())[2]).cuda()
+        h = _gelu(xv @ w1[g].t() + b1[g].double()).to(torch.bfloat16)
+        hv = torch.from_numpy(quantize_ref(h.double().cpu().numpy())[2]).cuda()
+        y[p:q] = hv @ w2[g].t() + b2[g].double()
+        mag[p:q] = hv.abs() @ w2[g].abs().t() + b2[g].abs().double()
+        top = max(top, h.abs().max().item())
+    return y, mag, top
+
+
+def _check_ffn(got, x, w1, b1, w2, b2, offsets):
+    W1, W2 = _values(w1), _values(w2)
+    y, mag, top = _plain_ffn(x, W1, b1, W2, b2, offsets)
+    # hidden values next to a border of the 4-bit grid may round to its other side: each moves by at most half its block's
+    # largest value; their share is the fp32 sums' error over the grid's spacing, about 1e-6: allow three in a row's reduction
+    flips = 3 * W2.abs().max().item() * top / 2
+    assert_within(got, y, bound(y, mag, W2.shape[2], torch.float32) + flips)
+
+
+@pytest.mark.parametrize('rows,e,c,seed', [(700, 8, 96, 1), (12, 4, 64, 2), (2500, 3, 136, 3)])
+@pytest.mark.parametrize('dtype', ['fp32', 'fp16'])
+def test_expert_ffn(rows, e, c, seed, dtype):
+    from sm3det_amd import mx4
+    x = _rows(seed, rows, c, DT[dtype], spread=1)
+    w1 = mx4.quantize(_rows(seed + 1, e * 4 * c, c, torch.float32, spread=1).view(e, 4 * c, c) * c ** -0.5)
+    w2 = mx4.quantize(_rows(seed + 2, e * c, 4 * c, torch.float32, spread=1).view(e, c, 4 * c) * (4 * c) ** -0.5)
+    b1, b2 = _rows(seed + 3, e, 4 * c, torch.float32, spread=1), _rows(seed + 4, e, c, torch.float32, spread=1)
+    offsets = ragged(seed, rows, e, tail=rows // 20)
+    off = torch.tensor(offsets, dtype=torch.int32, device='cuda')
+    got = mx4.expert_ffn(x, w1, b1, w2, b2, off)
+    assert got.dtype == torch.float32
+    _check_ffn(got, x, w1, b1, w2, b2, offsets)
+
+
+def test_backbone_with_quantised_experts(monkeypatch):
+    """every MoE block of the fixture's backbone in evaluation: the experts' inputs and outputs are caught and checked, the
+    rest of the forward is the full-precision one"""
+    from sm3det_amd import mx4
+    from sm3det_amd._lib import SM3Error
+    from sm3det_amd.convnext_moe import ConvNeXt_moe_MultiInput, MoE_layer
+    from tests.moe_common import load_fixture
+    fx = load_fixture('moe_e4k2')
+    net = ConvNeXt_moe_MultiInput(**fx['cfg'])
+    net.load_state_dict(fx['state_dict'])
+    net = net.cuda()
+    with pytest.raises(SM3Error):
+        mx4.quantize_experts(net.train())
+    net.eval()
+    x = fx['x'].cuda()
+    with torch.no_grad():
+        full = net(x, ['single'])
+    layers = [m for m in net.modules() if isinstance(m, MoE_layer)]
+    assert mx4.quantize_experts(net) == len(layers) > 0
+    caught = []
+    ffn = mx4.expert_ffn
+
+    def spy(xs, w1, b1, w2, b2, offsets):
+        y = ffn(xs, w1, b1, w2, b2, offsets)
+        caught.append((xs, w1, b1, w2, b2, offsets, y))
+        return y
+    monkeypatch.setattr(mx4, 'expert_ffn', spy)
+    with torch.no_grad():
+        outs = net(x, ['single'])
+    assert len(caught) == len(layers)
+    for (xs, w1, b1, w2, b2, offsets, y), m in zip(caught, layers):
+        assert w1.shape == m.w1.shape and w2.shape == m.w2.shape
+        _check_ffn(y, xs, w1, b1, w2, b2, offsets.tolist())
+    for a, b in zip(outs[0], full[0]):
+        assert a.shape == b.shape and torch.isfinite(a).all()
+    assert not torch.equal(outs[0][-1], full[0][-1])  # (stages without MoE blocks are the same)
+    with pytest.raises(SM3Error):  # a gradient would be needed
+        net(x, ['single'])
+    for again in (lambda: mx4.restore_experts(net), lambda: net.load_state_dict(fx['state_dict']), lambda: net.train().eval(),
+                  lambda: net.cuda()):
+        mx4.quantize_experts(net)
+        again()
+        with torch.no_grad():
+            back = net(x, ['single'])
+        assert all(torch.equal(a, b) for a, b in zip(back[0], full[0]))

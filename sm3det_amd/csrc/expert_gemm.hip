@@ -8,8 +8,21 @@ namespace {
 
 template <int KIND, int MODE>
 void launch_mode(const Params& P, const Plan& pl, hipStream_t st) {
-  if (MODE != M_TN && pl.bm == 32) tile_kernel<KIND, MODE == M_TN ? M_NT : MODE, 32, 128, 1, 4, 2><<<grid_of(pl, 3), 256, 0, st>>>(P);
-  else tile_kernel<KIND, MODE, 128, 128, 2, 2, 2><<<grid_of(pl, 2), 256, 0, st>>>(P);
+  if constexpr (MODE != M_TN) {
+    if (pl.coarse) {
+      Params Q = P;
+      Q.phase = 1;
+      tile_kernel<KIND, MODE, 256, 256, 2, 4, 2><<<grid_of(pl, 1), 512, 0, st>>>(Q);
+      Q.phase = 2;
+      tile_kernel<KIND, MODE, 128, 128, 2, 2, 1, 4><<<kNumCU, 256, 0, st>>>(Q);
+      return;
+    }
+    if (pl.bm == 32) {
+      tile_kernel<KIND, MODE, 32, 128, 1, 4, 2><<<grid_of(pl, 3), 256, 0, st>>>(P);
+      return;
+    }
+  }
+  tile_kernel<KIND, MODE, 128, 128, 2, 2, 2><<<grid_of(pl, 2), 256, 0, st>>>(P);
 }
 
 template <int KIND>

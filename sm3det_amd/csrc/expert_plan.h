@@ -15,6 +15,7 @@ struct Plan {
   int bm, bn;          // tile
   long mtiles, per_xcd;  // row tiles; jobs of one XCD
   int ntiles, splits;  // NT / NN: slices of the reduction
+  bool coarse;         // NT / NN: 256 x 256 tiles, the last partial round in quarters
   long unit_rows, units;  // TN: reduction rows per work unit
   size_t part_bytes, bsum_bytes;
   // copies of the operands made first: padded rows (16-bit), packed rows (4-bit; codes, then scales)
@@ -89,6 +90,16 @@ inline Plan plan_tiles(const sm3_expert_desc* d, bool mx4) {
   const long per_expert = d->rows / (d->num_groups < d->rows ? d->num_groups : d->rows > 0 ? d->rows : 1);
   p.bm = per_expert <= 48 ? 32 : 128;
   p.bn = 128;
+  // Long reductions over many tiles: 256 x 256 tiles move half the bytes per product through L2 (what bounds 128 x 128 ones there:
+  // 16384 rows, 8 experts, 4096 x 1024 174 -> 150 us, its input gradient 161 us either way), but a partial last round costs a
+  // whole one, so that one runs in quarters in a second launch.  Short ones (4 steps) gain nothing: 62 against 64 us.
+  const long red_steps = ((mx4 ? (d->red + 127) / 128 * 64 : d->red * 2L) + kStepBytes - 1) / kStepBytes;
+  const long some = d->offsets ? (d->num_groups < d->rows ? d->num_groups : d->rows) / 2 : 0;  // half a tile is lost per expert
+  const long expected = ((d->rows + 255) / 256 + some) * ((d->cols + 255L) / 256);
+  if (!mx4 && red_steps >= 16 && expected >= kNumCU && d->cols % 256 == 0) {
+    p.coarse = true;
+    p.bm = p.bn = 256;
+  }
   p.ntiles = (d->cols + p.bn - 1) / p.bn;
   p.mtiles = row_tiles(d->rows, d->num_groups, grouped, p.bm);
   p.splits = 1;

@@ -59,6 +59,7 @@ struct Params {
   int G;
   long S;
   int ntiles;                     // column tiles
+  int phase;                      // NT / NN: 0 all tiles; 1 the whole rounds of coarse tiles, 2 what they leave (see Jobs)
   int splits;                     // NT / NN: slices of the reduction; > 1: fp32 partials (splits, S, cols) in `part`
   long unit_rows;                 // TN: reduction rows per work unit
   float* part;                    // fp32 partials, or null: the result goes straight to `out`
@@ -85,7 +86,9 @@ struct Jobs {
   // BM, BN: output tile; row tiles are BM rows (NT / NN) or a work unit of unit_rows reduction rows (TN) with `mper` tiles each
   template <bool TN, int BM, int BN>
   __device__ __forceinline__ void init(const Params& P) {
-    const int bm = TN ? (int)P.unit_rows : BM;
+    constexpr int kCoarse = 256;  // tile of the rounds that a second launch finishes (phases 1 and 2, NT / NN)
+    const bool rest = !TN && P.phase == 2;
+    const int bm = TN ? (int)P.unit_rows : rest ? kCoarse : BM;
     const unsigned mper = TN ? (unsigned)(P.rows_out + BM - 1) / BM : 1u;  // TN: row tiles of a unit
     const int lane = threadIdx.x & 63, S = (int)P.S;
     const auto clamp = [&](int v) { return v < 0 ? 0 : v > S ? S : v; };
@@ -106,18 +109,25 @@ struct Jobs {
     const unsigned ntiles = (unsigned)P.ntiles, mtiles = (unsigned)(owned + behind + before);
     const unsigned stride = gridDim.x / kNumXCD, xcd = blockIdx.x % kNumXCD, slot = blockIdx.x / kNumXCD;
     unsigned t;
+    int quarter = 0;
     if constexpr (!TN) {
-      const unsigned tiles = mtiles * ntiles, jobs = tiles * (unsigned)P.splits;
+      const unsigned tiles = mtiles * ntiles;
+      // phase 1 runs whole rounds of one coarse tile per CU (and a last one that is at least a quarter full), phase 2 cuts the
+      // tiles that are left into four, one quarter per CU
+      const unsigned over = tiles % kNumCU, coarse = over > kNumCU / 4 ? tiles : tiles - over;
+      const unsigned jobs = P.phase == 0 ? tiles * (unsigned)P.splits : rest ? (tiles - coarse) * 4u : coarse;
       const unsigned per = (jobs + kNumXCD - 1) / kNumXCD;
       const unsigned begin = xcd * per, limit = begin + per < jobs ? begin + per : jobs;
       const unsigned mine = begin + slot, job = mine + lane * stride;
       count = mine < limit ? (int)((limit - mine + stride - 1) / stride) : 0;  // (<= kMaxJobs: the grid is made for it)
-      const unsigned z = job / tiles, lin = job - z * tiles;  // (lanes behind the last job compute something nobody reads)
+      const unsigned tile = rest ? coarse + job / 4u : job;
+      const unsigned z = tiles ? tile / tiles : 0u, lin = tile - z * tiles;  // (lanes behind the last job: nobody reads theirs)
       const unsigned band = lin / (4u * ntiles), in = lin - band * 4u * ntiles;
       const unsigned left = mtiles - band * 4u, deep = left < 4u ? (left ? left : 1u) : 4u;
       const unsigned nt = in / deep;
       t = band * 4u + (in - nt * deep);
-      col0 = (int)(nt * BN);
+      quarter = rest ? (int)(job & 3u) : 0;
+      col0 = (int)(nt * (rest ? kCoarse : BN)) + (quarter >> 1) * BN;
       prow0 = 0;
       unit = (int)z;
     } else {
@@ -218,6 +228,15 @@ struct Jobs {
     }
     rows = end_row - row0;
     rows = rows < 0 ? 0 : rows > bm ? bm : rows;
+    if (rest) {  // this quarter of the coarse tile, if it has one
+      row0 += (quarter & 1) * BM;
+      rows -= (quarter & 1) * BM;
+      rows = rows < 0 ? 0 : rows > BM ? BM : rows;
+      if (rows == 0 || col0 >= P.cols) {
+        g = -1;
+        rows = 0;
+      }
+    }
     __builtin_amdgcn_s_waitcnt(0x0f70);  // (nothing of this is in flight when the loader starts to count its own loads)
   }
 };
@@ -245,9 +264,12 @@ __device__ __forceinline__ void dma4(unsigned lds, unsigned voff, v4i desc) {
 }
 // this wave's direct loads have landed and its LDS reads are done; after the barrier everybody's.  (The builtin, not asm: the
 // compiler then knows that its own loads and stores are complete too and inserts no waits for them into the loop.)
+// All but the LATER loads issued last (the steps behind).
+template <int LATER>
 __device__ __forceinline__ void wait_and_sync() {
+  static_assert(LATER < 64, "six bits");
   asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+  __builtin_amdgcn_s_waitcnt(0x0070 | (LATER & 15) | (LATER >> 4) << 14);  // vmcnt(LATER) lgkmcnt(0)
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
@@ -449,7 +471,7 @@ __device__ __forceinline__ void for_each(F f) { for_each_of(std::make_integer_se
 //     round 0: multiply f0 | read f1 from buffer i
 //     wait for the loads of step i + 1 (issued a whole step ago), barrier
 //     round 1: multiply f1 | read f0 from buffer i + 1 | start loading step i + 2 into buffer i
-template <int KIND, int MODE, int BM, int BN, int WM, int WN, int MINW>
+template <int KIND, int MODE, int BM, int BN, int WM, int WN, int MINW, int NB = 2>
 __global__ void __launch_bounds__(WM * WN * 64, MINW) tile_kernel(const Params P) {
   constexpr int WAVES = WM * WN, TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
   constexpr bool PCOL = MODE == M_TN, QCOL = MODE != M_NT;
@@ -459,9 +481,10 @@ __global__ void __launch_bounds__(WM * WN * 64, MINW) tile_kernel(const Params P
   constexpr int NS = KIND == K_MX4 ? ((BM + BN) / 32 + WAVES - 1) / WAVES : 0;  // scale pieces of a wave: 32 rows x 8 bytes each
   constexpr int kScales = NS * WAVES * 256;
   constexpr int kBuf = kTile + kScales;
-  constexpr int kStage = 8 * (TN * 4 + 16);  // epilogue: 8 rows of a wave's columns
+  constexpr int SR = NB == 2 ? 8 : 4;                // epilogue for rows without 16-byte stores: SR rows of a wave's columns
+  constexpr int kStage = SR * (TN * 4 + 16);
   constexpr int kBias = MODE == M_TN ? 0 : 4 * BN * 4 + 256;  // bias rows of four jobs (the loader is at most two ahead)
-  __shared__ __attribute__((aligned(1024))) char lds[2 * kBuf + WAVES * kStage + kBias];
+  __shared__ __attribute__((aligned(1024))) char lds[NB * kBuf + WAVES * kStage + kBias];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -497,7 +520,7 @@ __global__ void __launch_bounds__(WM * WN * 64, MINW) tile_kernel(const Params P
   lq.init(wave, lane, P.ldq);
   constexpr int ND = lp.N + lq.N + NS;
   const unsigned base = __builtin_amdgcn_readfirstlane((int)lds_address(lds));
-  char* const bias_lds = lds + 2 * kBuf + WAVES * kStage;
+  char* const bias_lds = lds + NB * kBuf + WAVES * kStage;
 
   int lj = 0, lit = 0, lnum = -1;  // job being loaded, its step, its ordinal among the jobs that load anything
   Job lw{};
@@ -670,22 +693,20 @@ __global__ void __launch_bounds__(WM * WN * 64, MINW) tile_kernel(const Params P
     }
   };
 
+  constexpr int NL = ND + (MODE == M_TN ? 0 : 1);  // loads of a wave and step
   enter();
   if (more) {
-    aim();
-    aim_scales();
 #pragma unroll
-    for (int d = 0; d < ND; d++) dma(base, d);
-    aim_bias();
-    dma_bias();
-    advance();
-    aim();
-    aim_scales();
+    for (int n = 0; n < NB; n++) {
+      if (n) advance();
+      aim();
+      aim_scales();
+      aim_bias();
 #pragma unroll
-    for (int d = 0; d < ND; d++) dma(base + kBuf, d);
-    aim_bias();
-    dma_bias();
-    wait_and_sync();
+      for (int d = 0; d < ND; d++) dma(base + n * kBuf, d);
+      dma_bias();
+    }
+    wait_and_sync<(NB - 1) * NL>();
 #pragma unroll
     for (int r = 0; r < NR; r++) {
       read(lds, 0, r);
@@ -717,16 +738,17 @@ __global__ void __launch_bounds__(WM * WN * 64, MINW) tile_kernel(const Params P
       aim_bias();
       __builtin_amdgcn_sched_barrier(0);
       round(std::integral_constant<int, 0>{}, lds + off, 0);
-      wait_and_sync();
+      wait_and_sync<(NB - 2) * NL>();
       __builtin_amdgcn_sched_barrier(0);
-      round(std::integral_constant<int, 1>{}, lds + (kBuf - off), base + off);
+      const unsigned next = off == (NB - 1) * kBuf ? 0u : off + kBuf;
+      round(std::integral_constant<int, 1>{}, lds + next, base + off);
       if constexpr (KIND == K_MX4) {
 #pragma unroll
         for (int j = 0; j < FN; j++) qs[0][j] = qs[1][j];
 #pragma unroll
         for (int i = 0; i < FM; i++) ps[0][i] = ps[1][i];
       }
-      off = kBuf - off;
+      off = next;
     }
 
     int lane = threadIdx.x & 63;  // (opaque: what follows is computed here and not kept in registers through the loop)
@@ -806,9 +828,9 @@ __global__ void __launch_bounds__(WM * WN * 64, MINW) tile_kernel(const Params P
       });
       continue;
     }
-    // Rows that allow no 16-byte stores: 8 rows at a time go through this wave's own strip of LDS; a lane then holds eight
+    // Rows that allow no 16-byte stores: SR rows at a time go through this wave's own strip of LDS; a lane then holds eight
     // consecutive columns of a row.  (The loop is not unrolled: code for all of it would not stay in the instruction cache.)
-    constexpr int LR = TN / 8, PASS = 64 / LR > 8 ? 1 : 8 * LR / 64;  // lanes per row; passes over 8 rows
+    constexpr int LR = TN / 8, PASS = 64 / LR > SR ? 1 : SR * LR / 64;  // lanes per row; passes over SR rows
     constexpr int pitch = TN * 4 + 16;                               // (16 bytes between the rows move their banks apart)
     const int crow = lane / LR, ccol = lane % LR * 8, n = w.col0 + wn * TN + ccol;
     float bias[8] = {};
@@ -820,16 +842,16 @@ __global__ void __launch_bounds__(WM * WN * 64, MINW) tile_kernel(const Params P
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
       }
     }
-    char* const stage = lds + 2 * kBuf + wave * kStage;
+    char* const stage = lds + NB * kBuf + wave * kStage;
     const int have = P.cols - n;
-    for (int half = 0; half < 2 * FM; half++) {
-      const int orow = orow0 + half * 8;
+    for (int strip = 0; strip < 16 / SR * FM; strip++) {
+      const int orow = orow0 + strip * SR;
       if (orow >= olim) break;
-      for_each<FM>([&](auto I) {  // (the accumulators are registers: their indexes have to be constants)
+      for_each<FM>([&](auto I) {
         constexpr int i = decltype(I)::value;
-        if (half >> 1 == i && (lane >> 3 & 1) == (half & 1)) {
+        if (strip / (16 / SR) == i && (lane & 15) / SR == strip % (16 / SR)) {
 #pragma unroll
-          for (int j = 0; j < FN; j++) *(v4f*)(stage + (lane & 7) * pitch + (j * 16 + 4 * (lane >> 4)) * 4) = acc[i][j];
+          for (int j = 0; j < FN; j++) *(v4f*)(stage + lane % SR * pitch + (j * 16 + 4 * (lane >> 4)) * 4) = acc[i][j];
           asm volatile("; rows %0" ::"n"(i * 16));  // (keeps the branches' ends apart: merged, they would index acc at run time)
         }
       });
@@ -837,7 +859,7 @@ __global__ void __launch_bounds__(WM * WN * 64, MINW) tile_kernel(const Params P
 #pragma unroll
       for (int c = 0; c < PASS; c++) {
         const int row = crow + c * (64 / LR);
-        if (row < 8 && orow + row < olim && have > 0) {
+        if (row < SR && orow + row < olim && have > 0) {
           const v4f lo = *(const v4f*)(stage + row * pitch + ccol * 4), hi = *(const v4f*)(stage + row * pitch + ccol * 4 + 16);
           float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 #pragma unroll

@@ -90,13 +90,14 @@ inline Plan plan_tiles(const sm3_expert_desc* d, bool mx4) {
   const long per_expert = d->rows / (d->num_groups < d->rows ? d->num_groups : d->rows > 0 ? d->rows : 1);
   p.bm = per_expert <= 48 ? 32 : 128;
   p.bn = 128;
-  // Long reductions over many tiles: 256 x 256 tiles move half the bytes per product through L2 (what bounds 128 x 128 ones there:
-  // 16384 rows, 8 experts, 4096 x 1024 174 -> 150 us, its input gradient 161 us either way), but a partial last round costs a
-  // whole one, so that one runs in quarters in a second launch.  Short ones (4 steps) gain nothing: 62 against 64 us.
+  // Much work per CU: 256 x 256 tiles move half the bytes per product through L2 (16384 rows, 8 experts, 4096 x 1024: 174 -> 149 us,
+  // its input gradient 161 -> 148 us), but a partial last round costs a whole one, so that one runs in quarters in a second
+  // launch.  With one round of a short reduction the second launch costs more than the tile gains (65536 rows, reduction
+  // 1024 to 256 columns: 54 -> 61 us).
   const long red_steps = ((mx4 ? (d->red + 127) / 128 * 64 : d->red * 2L) + kStepBytes - 1) / kStepBytes;
   const long some = d->offsets ? (d->num_groups < d->rows ? d->num_groups : d->rows) / 2 : 0;  // half a tile is lost per expert
   const long expected = ((d->rows + 255) / 256 + some) * ((d->cols + 255L) / 256);
-  if (!mx4 && red_steps >= 16 && expected >= kNumCU && d->cols % 256 == 0) {
+  if (!mx4 && expected / kNumCU * red_steps >= 48 && red_steps >= 8 && d->cols % 256 == 0) {
     p.coarse = true;
     p.bm = p.bn = 256;
   }

@@ -252,6 +252,12 @@ __device__ __forceinline__ v4i descriptor(const void* base, long bytes) {
   return r;
 }
 
+__device__ __forceinline__ void move(v4i& desc, long by) {
+  const unsigned long long a = ((unsigned long long)(unsigned)desc[1] << 32 | (unsigned)desc[0]) + by;
+  desc[0] = (int)(unsigned)a;
+  desc[1] = (int)(unsigned)(a >> 32);
+}
+
 // 64 lanes x 16 (4) bytes from base + voff to LDS byte address `lds` + lane * 16 (4).  No result register; the caller waits
 // with wait_and_sync() before anything reads the LDS bytes.
 __device__ __forceinline__ void dma16(unsigned lds, unsigned voff, v4i desc) {
@@ -290,18 +296,18 @@ struct Loader {
   static constexpr int N = BX / 8 / WAVES;
   static_assert(BX / 8 % WAVES == 0 && N >= 1, "every wave loads the same number of 1 KB pieces");
   unsigned voff[N];
-  int gran;  // row operand: this lane's granule of the step (loop tail)
-  v4i desc;  // of the step being loaded
-  unsigned cut;
+  int gran;   // row operand: this lane's granule of a step
+  v4i desc;   // of the step being loaded: advanced from step to step, so that a step costs a handful of scalar instructions
+  bool tail;  // row operand: the step is the reduction's last and part-filled, voff of the lanes behind its end is out of range
 
   __device__ __forceinline__ void init(int wave, int lane, long ld) {
+    tail = false;
+    gran = (lane & 7) ^ (lane >> 3);
 #pragma unroll
     for (int i = 0; i < N; i++) {
       const int piece = wave * N + i;
       if constexpr (!COL) {
-        const int row = piece * 8 + (lane >> 3);
-        gran = (lane & 7) ^ (lane >> 3);
-        voff[i] = (unsigned)(row * ld) + gran * 16;
+        voff[i] = (unsigned)((piece * 8 + (lane >> 3)) * ld) + gran * 16;
       } else {
         constexpr int GR = BX / 8, RP = 64 / GR;  // granules per row, rows per piece
         const int row = piece * RP + lane / GR;
@@ -309,14 +315,21 @@ struct Loader {
       }
     }
   }
-  // left: bytes (row operand) of the reduction that remain from this step on; bytes <= 0: nothing is read, zeros arrive
-  __device__ __forceinline__ void aim(const char* base, long bytes, long left) {
+  // bytes <= 0: nothing is read, zeros arrive
+  __device__ __forceinline__ void start(const char* base, long bytes) {
     desc = descriptor(base, bytes);
-    cut = (!COL && gran * 16 >= left) ? kOutOfRange : 0u;
+    if (!COL && tail) {
+#pragma unroll
+      for (int i = 0; i < N; i++) voff[i] &= ~kOutOfRange;
+      tail = false;
+    }
   }
-  __device__ __forceinline__ void piece(unsigned lds, int wave, int i) const {
-    dma16(lds + (wave * N + i) * 1024, COL ? voff[i] : (voff[i] | cut), desc);
+  __device__ __forceinline__ void cut(int left) {  // row operand: fewer than kStepBytes remain
+    tail = true;
+#pragma unroll
+    for (int i = 0; i < N; i++) voff[i] |= gran * 16 >= left ? kOutOfRange : 0u;
   }
+  __device__ __forceinline__ void piece(unsigned lds, int wave, int i) const { dma16(lds + (wave * N + i) * 1024, voff[i], desc); }
 };
 
 // ---- fragments ----------------------------------------------------------------------------------------------------
@@ -525,50 +538,9 @@ __global__ void __launch_bounds__(WM * WN * 64, MINW) tile_kernel(const Params P
   int lj = 0, lit = 0, lnum = -1;  // job being loaded, its step, its ordinal among the jobs that load anything
   Job lw{};
   bool more = true;
-  const char *pb = P.p, *qb = P.q;                 // where the step starts
-  const unsigned char *psb = P.ps, *qsb = P.qs;    // MX4: scale bytes
-  int kleft = 0, rleft = 0;                        // row operand: bytes, column operand: rows of the reduction that remain
-  auto enter = [&]() {  // the first job from lj on that has steps
-    for (;; lj++) {
-      if (lj >= jobs.count) {
-        more = false;
-        return;
-      }
-      lw = job_of(lj);
-      if (lw.s0 < lw.s1) break;
-    }
-    lit = lw.s0;
-    lnum++;
-    const long k = (long)lit * kStepBytes, r = (long)lit * kStepRed;
-    if constexpr (MODE == M_TN) {
-      pb = P.p + (lw.row0 + r) * P.ldp + (long)lw.prow0 * 2;
-      qb = P.q + (lw.row0 + r) * P.ldq + (long)lw.col0 * 2;
-      rleft = lw.rows - (int)r;
-    } else {
-      pb = P.p + (long)lw.row0 * P.ldp + k;
-      kleft = (int)(P.red - k);
-      if constexpr (MODE == M_NN) {
-        qb = P.q + lw.g * P.strideq + r * P.ldq + (long)lw.col0 * 2;
-        rleft = (int)(P.qred - r);
-      } else {
-        qb = P.q + lw.g * P.strideq + (long)lw.col0 * P.ldq + k;
-      }
-    }
-    if constexpr (KIND == K_MX4) {
-      psb = P.ps + (long)lw.row0 * P.ldps + lit * 8;
-      qsb = P.qs + lw.g * P.strideqs + (long)lw.col0 * P.ldqs + lit * 8;
-    }
-  };
-  auto aim = [&]() {  // descriptors of the step at (lw, lit); nothing is left: empty ones (zeros arrive)
-    const int qrows = P.cols - lw.col0 < BN ? P.cols - lw.col0 : BN;
-    const int n = rleft < kStepRed ? rleft : kStepRed;
-    const int pw = (P.rows_out * 2 + 15) & ~15, qw = (P.cols * 2 + 15) & ~15;
-    if constexpr (PCOL) lp.aim(pb, more ? (n - 1) * (int)P.ldp + pw - lw.prow0 * 2 : 0, 0);
-    else lp.aim(pb, more ? (lw.rows - 1) * (int)P.ldp + kleft : 0, kleft);
-    if constexpr (QCOL) lq.aim(qb, more ? (n - 1) * (int)P.ldq + qw - lw.col0 * 2 : 0, 0);
-    else lq.aim(qb, more ? (qrows - 1) * (int)P.ldq + kleft : 0, kleft);
-  };
-  // scale pieces (no branches here: they would tear the rounds' instructions apart)
+  int kleft = 0, rleft = 0;  // row operand: bytes, column operand: rows of the reduction that remain
+  const int pw = (P.rows_out * 2 + 15) & ~15, qw = (P.cols * 2 + 15) & ~15;  // bytes of a column operand's rows
+  // MX4: scale pieces
   unsigned svoff[NS ? NS : 1], scut = 0;
   v4i sdesc[NS ? NS : 1];
   if constexpr (KIND == K_MX4) {
@@ -578,25 +550,73 @@ __global__ void __launch_bounds__(WM * WN * 64, MINW) tile_kernel(const Params P
       svoff[c] = (unsigned)(row * (int)(i < BM / 32 ? P.ldps : P.ldqs)) + 4 * (lane & 1);
     }
   }
-  auto aim_scales = [&]() {
+  // the bias row of a job travels with its first step as one more piece (slot: the job's ordinal modulo 4; other steps load
+  // nothing into a fifth)
+  const int bes = P.bias_type == DT_F32 ? 4 : 2;
+  const unsigned bias_none = base + (unsigned)(bias_lds - lds) + 4 * (BN * 4);
+  unsigned bias_to = bias_none;
+  v4i bdesc = descriptor(P.bias, 0);
+
+  auto last_rows = [&]() {  // column operands: the rows of the step that exist
+    const int n = rleft < kStepRed ? rleft : kStepRed;
+    if constexpr (PCOL) lp.desc[2] = (n - 1) * (int)P.ldp + pw - lw.prow0 * 2;
+    if constexpr (QCOL) lq.desc[2] = (n - 1) * (int)P.ldq + qw - lw.col0 * 2;
+  };
+  auto last_bytes = [&]() {  // row operands: fewer than a step's bytes remain
+    if constexpr (!PCOL) lp.cut(kleft);
+    if constexpr (!QCOL) lq.cut(kleft);
+    if constexpr (KIND == K_MX4) scut = 4 * (lane & 1) >= kleft / 16 ? kOutOfRange : 0u;
+  };
+  auto enter = [&]() {  // the first job from lj on that has steps: descriptors of its first one
+    for (;; lj++) {
+      if (lj >= jobs.count) {  // nothing is left: empty descriptors (zeros arrive)
+        more = false;
+        lp.desc[2] = 0;
+        lq.desc[2] = 0;
+        bdesc[2] = 0;
+        bias_to = bias_none;
+        if constexpr (KIND == K_MX4) {
+#pragma unroll
+          for (int c = 0; c < NS; c++) sdesc[c][2] = 0;
+        }
+        return;
+      }
+      lw = job_of(lj);
+      if (lw.s0 < lw.s1) break;
+    }
+    lit = lw.s0;
+    lnum++;
+    const long k = (long)lit * kStepBytes, r = (long)lit * kStepRed;
+    const int qrows = P.cols - lw.col0 < BN ? P.cols - lw.col0 : BN;
+    kleft = (int)(P.red - k);
+    if constexpr (MODE == M_TN) {
+      rleft = lw.rows - (int)r;
+      lp.start(P.p + (lw.row0 + r) * P.ldp + (long)lw.prow0 * 2, 0);
+      lq.start(P.q + (lw.row0 + r) * P.ldq + (long)lw.col0 * 2, 0);
+    } else {
+      rleft = (int)(P.qred - r);
+      lp.start(P.p + (long)lw.row0 * P.ldp + k, (long)(lw.rows - 1) * P.ldp + kleft);
+      if constexpr (MODE == M_NN) lq.start(P.q + lw.g * P.strideq + r * P.ldq + (long)lw.col0 * 2, 0);
+      else lq.start(P.q + lw.g * P.strideq + (long)lw.col0 * P.ldq + k, (long)(qrows - 1) * P.ldq + kleft);
+    }
     if constexpr (KIND == K_MX4) {
-      const int have = kleft / 16, qrows = P.cols - lw.col0 < BN ? P.cols - lw.col0 : BN;
-      const int pbytes = (lw.rows - 1) * (int)P.ldps + have, qbytes = (qrows - 1) * (int)P.ldqs + have;
-      scut = 4 * (lane & 1) >= have ? kOutOfRange : 0u;
+      const unsigned char* psb = P.ps + (long)lw.row0 * P.ldps + lit * 8;
+      const unsigned char* qsb = P.qs + lw.g * P.strideqs + (long)lw.col0 * P.ldqs + lit * 8;
+      const long pbytes = (lw.rows - 1) * P.ldps + kleft / 16, qbytes = (qrows - 1) * P.ldqs + kleft / 16;
+      scut = 0;
 #pragma unroll
       for (int c = 0; c < NS; c++) {
         const int i = c * WAVES + wave;  // (pieces behind the last read nothing; their zeros go to padding)
-        const int bytes = i < BM / 32 ? pbytes : i < (BM + BN) / 32 ? qbytes : 0;
-        sdesc[c] = descriptor(i < BM / 32 ? psb : qsb, more ? bytes : 0);
+        sdesc[c] = descriptor(i < BM / 32 ? psb : qsb, i < BM / 32 ? pbytes : i < (BM + BN) / 32 ? qbytes : 0);
       }
     }
-  };
-  auto dma = [&](unsigned at, int d) {  // piece d of the step aimed at, into the buffer at LDS address `at`
-    if (d < lp.N) lp.piece(at, wave, d);
-    else if (d < lp.N + lq.N) lq.piece(at + BM * kStepBytes, wave, d - lp.N);
-    else if constexpr (KIND == K_MX4) {  // 8 scale bytes per row and step: 32 rows per instruction
-      const int c = d - lp.N - lq.N;
-      dma4(at + kTile + (c * WAVES + wave) * 256, svoff[c] | scut, sdesc[c]);
+    if constexpr (PCOL || QCOL) last_rows();
+    if constexpr (!PCOL) { if (kleft < kStepBytes) last_bytes(); }
+    if constexpr (MODE != M_TN) {
+      if (P.bias_lds && wave * 256 < BN * bes) {
+        bdesc = descriptor((const char*)P.bias + ((long)lw.g * P.cols + lw.col0) * bes, (long)(P.cols - lw.col0) * bes);
+        bias_to = base + (unsigned)(bias_lds - lds) + (lnum & 3) * (BN * 4) + wave * 256;
+      }
     }
   };
   auto advance = [&]() {  // to the next step (of the next job where this one ends)
@@ -604,28 +624,32 @@ __global__ void __launch_bounds__(WM * WN * 64, MINW) tile_kernel(const Params P
     if (++lit >= lw.s1) {
       lj++;
       enter();
-    } else {
-      if constexpr (PCOL) pb += kStepRed * P.ldp; else pb += kStepBytes;
-      if constexpr (QCOL) qb += kStepRed * P.ldq; else qb += kStepBytes;
-      kleft -= kStepBytes;
-      rleft -= kStepRed;
-      if constexpr (KIND == K_MX4) {
-        psb += 8;
-        qsb += 8;
+      return;
+    }
+    move(lp.desc, PCOL ? kStepRed * P.ldp : kStepBytes);
+    move(lq.desc, QCOL ? kStepRed * P.ldq : kStepBytes);
+    if constexpr (!PCOL) lp.desc[2] -= kStepBytes;
+    if constexpr (!QCOL) lq.desc[2] -= kStepBytes;
+    kleft -= kStepBytes;
+    rleft -= kStepRed;
+    if constexpr (KIND == K_MX4) {
+#pragma unroll
+      for (int c = 0; c < NS; c++) {
+        move(sdesc[c], 8);
+        sdesc[c][2] = sdesc[c][2] > 8 ? sdesc[c][2] - 8 : 0;
       }
     }
+    if constexpr (PCOL || QCOL) { if (rleft < kStepRed) last_rows(); }
+    if constexpr (!PCOL) { if (kleft < kStepBytes) last_bytes(); }
+    bdesc[2] = 0;
+    bias_to = bias_none;
   };
-  // the bias row of a job travels with its first step as one more piece (slot: the job's ordinal modulo 4; other steps load
-  // nothing into a fifth)
-  const int bes = P.bias_type == DT_F32 ? 4 : 2;
-  unsigned bias_to = 0;
-  v4i bdesc = {};
-  auto aim_bias = [&]() {
-    if constexpr (MODE != M_TN) {
-      const bool now = P.bias_lds && more && lit == lw.s0 && wave * 256 < BN * bes;
-      const long at = ((long)lw.g * P.cols + lw.col0) * bes;
-      bdesc = descriptor((const char*)P.bias + at, now ? (long)(P.cols - lw.col0) * bes : 0);
-      bias_to = base + (unsigned)(bias_lds - lds) + (now ? (lnum & 3) * (BN * 4) + wave * 256 : 4 * (BN * 4));
+  auto dma = [&](unsigned at, int d) {  // piece d of the step, into the buffer at LDS address `at`
+    if (d < lp.N) lp.piece(at, wave, d);
+    else if (d < lp.N + lq.N) lq.piece(at + BM * kStepBytes, wave, d - lp.N);
+    else if constexpr (KIND == K_MX4) {  // 8 scale bytes per row and step: 32 rows per instruction
+      const int c = d - lp.N - lq.N;
+      dma4(at + kTile + (c * WAVES + wave) * 256, svoff[c] | scut, sdesc[c]);
     }
   };
   auto dma_bias = [&]() {
@@ -699,9 +723,6 @@ __global__ void __launch_bounds__(WM * WN * 64, MINW) tile_kernel(const Params P
 #pragma unroll
     for (int n = 0; n < NB; n++) {
       if (n) advance();
-      aim();
-      aim_scales();
-      aim_bias();
 #pragma unroll
       for (int d = 0; d < ND; d++) dma(base + n * kBuf, d);
       dma_bias();
@@ -733,9 +754,6 @@ __global__ void __launch_bounds__(WM * WN * 64, MINW) tile_kernel(const Params P
       // (everything with branches stands before the rounds: the multiplications are free of side effects, and the compiler
       // would move those of a round behind a branch that follows it, away from the loads they are to cover)
       advance();
-      aim();
-      aim_scales();
-      aim_bias();
       __builtin_amdgcn_sched_barrier(0);
       round(std::integral_constant<int, 0>{}, lds + off, 0);
       wait_and_sync<(NB - 2) * NL>();

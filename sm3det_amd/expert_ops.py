@@ -13,11 +13,11 @@ counts): the host never reads them, so calls are free of synchronisation and can
 * rows of no expert (before ``offsets[0]``, behind ``offsets[-1]``): y and dx are zero there and they enter no gradient.
   Offsets outside [0, rows] are clamped, decreasing ones made monotone.
 * an expert without rows gets zero gradients (never an uninitialised one).
+* first derivatives only: the gradients themselves carry no graph.
 * gradients do not depend on the order in which workgroups run: split reductions are added in a fixed order, no atomics.
 """
 import torch
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import _lib_backbone as LB
 from ._lib import SM3Error, check, lib, require_gpu
@@ -105,7 +105,6 @@ class _ExpertLinear(Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
         x, w, offsets = ctx.saved_tensors
         S, K = x.shape

@@ -138,7 +138,8 @@ class MoE_layer(nn.Module):
         self.last_expert_offsets = None  # device int32 (E+1): expert loads of the last forward (no sync)
         self.last_importance_load = None  # device fp32 (2E): [importance | load] of the last forward
         self.last_top_idx = None  # device int32 (T, min(k+1,E)): the routing of the last forward, best first
-        self._mx4 = None  # packed 4-bit (w1, w2) of mx4.quantize_experts; gone when the weights may change or move
+
+    _mx4 = None  # packed 4-bit (w1, w2) of mx4.quantize_experts; gone when the weights may change or move
 
     def experts(self):
         """what takes the place of the expert FFNs in this forward: None, or the 4-bit experts (evaluation only)"""

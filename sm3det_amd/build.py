@@ -15,10 +15,7 @@ CSRC = os.path.join(HERE, 'csrc')
 LIB = os.path.join(CSRC, 'libsm3det_hip.so')
 ARCH = 'gfx950'
 
-# packed fp32 instructions (v_pk_add / mul / fma_f32, which -O3 forms from scalar code by itself) stay off: some of their forms
-# have given wrong results on this hardware, with no error (the host pass warns that it does not know the feature: harmless)
-BASE_FLAGS = ['--offload-arch=' + ARCH, '-O3', '-std=c++17', '-fPIC', '-Wall', '-Wno-unused-function',
-              '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
+BASE_FLAGS = ['--offload-arch=' + ARCH, '-O3', '-std=c++17', '-fPIC', '-Wall', '-Wno-unused-function']
 # Per-file flags.  The detection ops must round exactly like the reference's scalar CPU code (bit-exact NMS),
 # so no FMA contraction there; the backbone kernels keep the default (-ffp-contract=fast-honor-pragmas).
 FILE_FLAGS = {

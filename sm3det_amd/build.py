@@ -18,7 +18,13 @@ ARCH = 'gfx950'
 BASE_FLAGS = ['--offload-arch=' + ARCH, '-O3', '-std=c++17', '-fPIC', '-Wall', '-Wno-unused-function']
 # Per-file flags.  The detection ops must round exactly like the reference's scalar CPU code (bit-exact NMS),
 # so no FMA contraction there; the backbone kernels keep the default (-ffp-contract=fast-honor-pragmas).
+# Packed fp32 instructions (v_pk_add / mul / fma_f32, which -O3 forms from scalar code by itself) stay off in these files: some of
+# their forms have given wrong results on this hardware, with no error (the host pass warns that it does not know the feature:
+# harmless).  The other files keep the code they were validated with: without packed instructions backbone.hip, moe_router.hip and
+# gemm_h16.hip round differently, and the full-size AMP fixture's routing and its cancelling temperature gradient move with them.
+NO_PACKED_FP32 = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 FILE_FLAGS = {
+    'expert_gemm.hip': NO_PACKED_FP32, 'mx4.hip': NO_PACKED_FP32, 'mx4_few.hip': NO_PACKED_FP32, 'mx4_gemm.hip': NO_PACKED_FP32,
     'ops_rotated.hip': ['-ffp-contract=off'],
     'deform_conv.hip': ['-ffp-contract=off'],
     'rpn.hip': ['-ffp-contract=off'],

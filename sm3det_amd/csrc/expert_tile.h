@@ -92,20 +92,69 @@ struct Jobs {
     const unsigned mper = TN ? (unsigned)(P.rows_out + BM - 1) / BM : 1u;  // TN: row tiles of a unit
     const int lane = threadIdx.x & 63, S = (int)P.S;
     const auto clamp = [&](int v) { return v < 0 ? 0 : v > S ? S : v; };
-    const auto tiles_of = [&](int len) { const int n = (len + bm - 1) / bm; return TN && n == 0 ? 1 : n; };
-    const auto ends_from = [&](int e) { return P.offsets ? P.offsets[1 + (e + lane < P.G ? e + lane : 0)] : S; };
-    int ends = ends_from(0);
-    const int raw = P.offsets ? P.offsets[0] : 0;
-    const int first = clamp(__builtin_amdgcn_readfirstlane(raw));
-    int last = first, owned = 0;  // rows and row tiles of experts
-    for (int e = 0; e < P.G; e++) {
-      if (e && (e & 63) == 0) ends = ends_from(e);
-      const int end = clamp(__builtin_amdgcn_readlane(ends, e & 63));
-      const int to = end > last ? end : last;
-      owned += tiles_of(to - last);
-      last = to;
+    const auto tiles_of = [&](int len) { return (int)((unsigned)(len + (unsigned)bm - 1u) / (unsigned)bm); };
+    const auto ends_from = [&](int e) { return P.offsets[1 + (e + lane < P.G ? e + lane : 0)]; };
+    // owned: row tiles of the experts; last: where the last expert ends.  An expert without rows has one (empty) unit in TN.
+    int first = 0, last = S, owned = tiles_of(S);
+    if (TN && owned == 0) owned = 1;
+    // up to 64 experts: lane e holds expert e's range and its share of the running count (TN: in the order of work)
+    const bool lanes = P.offsets != nullptr && P.G <= 64;
+    int from = 0, len = 0, n = 0, incl = 0, expert = lane, unit0 = 0;
+    const auto count_up = [&](int v) {
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(v, d);
+        v += lane >= d ? o : 0;
+      }
+      return v;
+    };
+    if (P.offsets != nullptr) {
+      const int ends = ends_from(0), raw = P.offsets[0];
+      first = clamp(__builtin_amdgcn_readfirstlane(raw));
+      if (lanes) {
+        int to = lane < P.G ? clamp(ends) : 0;
+        to = to < first ? first : to;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+          const int o = __shfl_up(to, d);
+          to = lane >= d && o > to ? o : to;
+        }
+        from = __shfl_up(to, 1);
+        if (lane == 0) from = first;
+        len = lane < P.G ? to - from : 0;
+        n = tiles_of(len);
+        if (TN && lane < P.G && n == 0) n = 1;
+        incl = count_up(n);
+        last = __builtin_amdgcn_readlane(to, 63);
+        owned = __builtin_amdgcn_readlane(incl, 63);
+        if (TN && P.part == nullptr) {  // longest expert first (ties: the lower index)
+          int rank = 0;
+          for (int e = 0; e < P.G; e++) {
+            const int l = __builtin_amdgcn_readlane(len, e);
+            rank += l > len || (l == len && e < lane) ? 1 : 0;
+          }
+          const int to_lane = 4 * (lane < P.G ? rank : lane);
+          unit0 = __builtin_amdgcn_ds_permute(to_lane, incl - n);
+          expert = __builtin_amdgcn_ds_permute(to_lane, lane);
+          from = __builtin_amdgcn_ds_permute(to_lane, from);
+          len = __builtin_amdgcn_ds_permute(to_lane, len);
+          n = __builtin_amdgcn_ds_permute(to_lane, n);
+          incl = count_up(n);
+        }
+      } else {
+        last = first;
+        owned = 0;
+        int held = ends;
+        for (int e = 0; e < P.G; e++) {
+          if (e && (e & 63) == 0) held = ends_from(e);
+          const int end = clamp(__builtin_amdgcn_readlane(held, e & 63));
+          const int to = end > last ? end : last, m = tiles_of(to - last);
+          owned += TN && m == 0 ? 1 : m;
+          last = to;
+        }
+      }
     }
-    const int behind = TN ? 0 : (S - last + bm - 1) / bm, before = TN ? 0 : (first + bm - 1) / bm;
+    const int behind = TN ? 0 : tiles_of(S - last), before = TN ? 0 : tiles_of(first);
     const unsigned ntiles = (unsigned)P.ntiles, mtiles = (unsigned)(owned + behind + before);
     const unsigned stride = gridDim.x / kNumXCD, xcd = blockIdx.x % kNumXCD, slot = blockIdx.x / kNumXCD;
     unsigned t;
@@ -160,69 +209,46 @@ struct Jobs {
     g = -1;
     row0 = 0;
     int end_row = 0;
-    if constexpr (TN) {
-      int at = 0, prev = first;
-      if (P.G <= 64) {
-        int from = 0, len = 0, unit0 = 0, rank = 0;  // lane e: expert e
-        for (int e = 0; e < P.G; e++) {
-          const int end = clamp(__builtin_amdgcn_readlane(ends, e)), to = end > prev ? end : prev;
-          if (lane == e) {
-            from = prev;
-            len = to - prev;
-            unit0 = at;
-          }
-          at += tiles_of(to - prev);
-          prev = to;
-        }
-        for (int e = 0; e < P.G; e++) {
-          const int l = __builtin_amdgcn_readlane(len, e);
-          rank += l > len || (l == len && e < lane) ? 1 : 0;
-        }
-        at = 0;
-        for (int r = 0; r < P.G; r++) {
-          const int e = __ffsll(__ballot(rank == r && lane < P.G)) - 1;
-          const int l = __builtin_amdgcn_readlane(len, e), f = __builtin_amdgcn_readlane(from, e);
-          const int u = __builtin_amdgcn_readlane(unit0, e), n = tiles_of(l);
-          if (t != ~0u && (int)t >= at && (int)t < at + n) {
-            g = e;
-            row0 = f + ((int)t - at) * bm;
-            end_row = f + l;
-            unit = u + (int)t - at;
-          }
-          at += n;
-        }
-      } else {
-        ends = ends_from(0);
-        for (int e = 0; e < P.G; e++) {
-          if (e && (e & 63) == 0) ends = ends_from(e);
-          const int end = clamp(__builtin_amdgcn_readlane(ends, e & 63));
-          const int to = end > prev ? end : prev, n = tiles_of(to - prev);
-          if (t != ~0u && (int)t >= at && (int)t < at + n) {
-            g = e;
-            row0 = prev + ((int)t - at) * bm;
-            end_row = to;
-            unit = (int)t;
-          }
-          at += n;
-          prev = to;
-        }
-      }
-    } else {
+    if constexpr (!TN) {  // rows of no expert, unless one is found below
       const int i = (int)t - owned;
       row0 = i < behind ? last + i * bm : (i - behind) * bm;
       end_row = i < behind ? S : first;
-      int at = 0, prev = first;
-      if (P.G > 64) ends = ends_from(0);
+    }
+    if (P.offsets == nullptr) {
+      if (t < (unsigned)owned) {
+        g = 0;
+        row0 = (int)t * bm;
+        end_row = S;
+        if (TN) unit = (int)t;
+      }
+    } else if (lanes) {
+      int e = 0;  // the lane whose running count first exceeds t
+#pragma unroll
+      for (int step = 32; step; step >>= 1) e += (unsigned)__shfl(incl, e + step - 1) <= t ? step : 0;
+      e = e < 63 ? e : 63;
+      const int at = (int)t - __shfl(incl - n, e), f = __shfl(from, e), l = __shfl(len, e), x = __shfl(expert, e);
+      const int u = __shfl(unit0, e);
+      if (t < (unsigned)owned) {
+        g = x;
+        row0 = f + at * bm;
+        end_row = f + l;
+        if (TN) unit = P.part == nullptr ? u + at : (int)t;
+      }
+    } else {
+      int at = 0, prev = first, held = ends_from(0);
       for (int e = 0; e < P.G; e++) {
-        if (e && (e & 63) == 0) ends = ends_from(e);
-        const int end = clamp(__builtin_amdgcn_readlane(ends, e & 63));
-        const int to = end > prev ? end : prev, n = tiles_of(to - prev);
-        if ((int)t >= at && (int)t < at + n) {
+        if (e && (e & 63) == 0) held = ends_from(e);
+        const int end = clamp(__builtin_amdgcn_readlane(held, e & 63));
+        const int to = end > prev ? end : prev;
+        int m = tiles_of(to - prev);
+        if (TN && m == 0) m = 1;
+        if (t != ~0u && (int)t >= at && (int)t < at + m) {
           g = e;
           row0 = prev + ((int)t - at) * bm;
           end_row = to;
+          if (TN) unit = (int)t;
         }
-        at += n;
+        at += m;
         prev = to;
       }
     }

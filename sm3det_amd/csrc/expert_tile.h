@@ -29,6 +29,7 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+typedef unsigned v4u __attribute__((ext_vector_type(4)));
 
 enum { DT_F32 = SM3_DT_F32, DT_F16 = SM3_DT_F16, DT_BF16 = SM3_DT_BF16 };
 enum { K_F16 = 0, K_BF16 = 1, K_MX4 = 2 };   // operand kinds
@@ -306,6 +307,26 @@ __device__ __forceinline__ void wait_and_sync() {
   asm volatile("" ::: "memory");
 }
 
+template <class T>
+__device__ __forceinline__ T* uniform(T* p) {
+  const unsigned long long a = (unsigned long long)p;
+  const unsigned lo = __builtin_amdgcn_readfirstlane((int)(unsigned)a), hi = __builtin_amdgcn_readfirstlane((int)(unsigned)(a >> 32));
+  return (T*)((unsigned long long)hi << 32 | lo);
+}
+
+// The same where AFTER stores may stand behind those loads (`stored`: they do).  Loads and stores of a wave complete in the order
+// of issue as far as the counter goes, so the loads are waited for without the stores.  The branch is inside the asm: one that
+// the compiler sees would split the rounds' blocks.
+template <int LATER, int AFTER>
+__device__ __forceinline__ void wait_and_sync(int stored) {
+  static_assert(LATER + AFTER < 64, "six bits");
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+  asm volatile("s_cmp_lg_u32 %0, 0\n\ts_waitcnt vmcnt(%1)\n\ts_cbranch_scc1 .Lloaded%=\n\ts_waitcnt vmcnt(%2)\n.Lloaded%=:"
+               :: "s"(__builtin_amdgcn_readfirstlane(stored)), "n"(LATER + AFTER), "n"(LATER) : "memory", "scc");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 __device__ __forceinline__ unsigned lds_address(const void* p) {
   return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
 }
@@ -457,12 +478,8 @@ __device__ __forceinline__ v4f bias4(const void* b, int type, long at, long most
 }
 
 __device__ __forceinline__ unsigned pack2(float a, float b, int type) {  // rounded to nearest even
-  if (type == DT_F16) {
-    const _Float16 x = (_Float16)a, y = (_Float16)b;
-    return (unsigned)__builtin_bit_cast(unsigned short, x) | (unsigned)__builtin_bit_cast(unsigned short, y) << 16;
-  }
-  const __bf16 x = (__bf16)a, y = (__bf16)b;
-  return (unsigned)__builtin_bit_cast(unsigned short, x) | (unsigned)__builtin_bit_cast(unsigned short, y) << 16;
+  if (type == DT_F16) return __builtin_bit_cast(unsigned, v2h{(_Float16)a, (_Float16)b});
+  return __builtin_bit_cast(unsigned, v2b{(__bf16)a, (__bf16)b});
 }
 
 // eight consecutive values of one row, `n` of them exist; wide: 16-byte stores are allowed (and n is a multiple of what one holds)
@@ -519,6 +536,7 @@ template <int KIND, int MODE, int BM, int BN, int WM, int WN, int MINW, int NB =
 __global__ void __launch_bounds__(WM * WN * 64, MINW) tile_kernel(const Params P) {
   constexpr int WAVES = WM * WN, TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
   constexpr bool PCOL = MODE == M_TN, QCOL = MODE != M_NT;
+  static_assert(FN % 2 == 0, "the epilogue takes blocks in pairs");
   static_assert(KIND != K_MX4 || MODE == M_NT, "4-bit operands: rows only");
   constexpr bool ACT = KIND == K_MX4;  // (the 16-bit products have no activation: their gradients would need its derivative)
   constexpr int kTile = (BM + BN) * kStepBytes;
@@ -768,6 +786,8 @@ __global__ void __launch_bounds__(WM * WN * 64, MINW) tile_kernel(const Params P
 
   unsigned off = 0;
   int num = -1;
+  constexpr int kStores = FM * FN / 2;  // at least so many stores end a tile ...
+  int stored = 0;                       // ... and one has ended since the last step (rows with 16-byte stores only)
   for (int cj = 0; cj < jobs.count; cj++) {
     const Job w = job_of(cj);
     if (MODE == M_TN && w.g < 0) continue;  // (the XCDs' shares of a unit's tiles are rounded up)
@@ -787,7 +807,8 @@ __global__ void __launch_bounds__(WM * WN * 64, MINW) tile_kernel(const Params P
       advance();
       __builtin_amdgcn_sched_barrier(0);
       round(std::integral_constant<int, 0>{}, lds + off, 0);
-      wait_and_sync<(NB - 2) * NL>();
+      wait_and_sync<(NB - 2) * NL, kStores>(stored);
+      stored = 0;
       __builtin_amdgcn_sched_barrier(0);
       const unsigned next = off == (NB - 1) * kBuf ? 0u : off + kBuf;
       round(std::integral_constant<int, 1>{}, lds + next, base + off);
@@ -845,36 +866,69 @@ __global__ void __launch_bounds__(WM * WN * 64, MINW) tile_kernel(const Params P
         }
         // waited for here, on this path: left to the first use, the compiler puts a wait for EVERY load into the next tile's loop
       }
-      const int g16 = lane >> 4, ncol = w.col0 + wn * TN;
-      for_each<FM>([&](auto I) {  // (the accumulators are registers: their indexes have to be constants)
-        constexpr int i = decltype(I)::value;
-        if (orow0 + i * 16 >= olim) return;
-        const int orow = orow0 + i * 16 + (lane & 15);
-        char* const row = (char*)out + (first + orow) * P.cols * (type == DT_F32 ? 4 : 2);
+      // One straight run of instructions per result type, with the activation or without: the descriptor's range check drops the
+      // rows behind olim, an address out of range the columns behind the last (65536 x 1024 x 256, bf16: a tile's end took
+      // 6200 cycles with branches, 2600 without; 4-bit 16384 x 2048 x 512 with GELU 53 -> 43 us).
+      const auto emit = [&](auto type_of, auto act_of) {
+        constexpr int type = decltype(type_of)::value, es = type == DT_F32 ? 4 : 2;
+        const int g16 = lane >> 4, ncol = w.col0 + wn * TN, pitch = P.cols * es;
+        const int have = P.cols - ncol, rows = olim - orow0 < TM ? olim - orow0 : TM;
+        const auto to = __builtin_amdgcn_make_buffer_rsrc(
+            uniform((char*)out + (first + orow0) * pitch + (long)ncol * es), (short)0,
+            __builtin_amdgcn_readfirstlane(rows > 0 && have > 0 ? (rows - 1) * pitch + have * es : 0), 0x00020000);
 #pragma unroll
-        for (int j = 0; j < FN; j += 2) {
-          float v[8];
+        for (int j = 0; j < FN; j++)  // (opaque: the sums would else be moved in front of the choice of the type, all at once)
+          asm volatile("; results of type %1" : "+v"(bias[j]) : "n"(type + 8 * decltype(act_of)::value));
+        unsigned at[FN];  // of the columns of block j (16 bits: of blocks j and j + 1)
 #pragma unroll
-          for (int r = 0; r < 4; r++) {
-            v[r] = acc[i][j][r] + bias[j][r];
-            v[r + 4] = acc[i][j + 1][r] + bias[j + 1][r];
-          }
-          if (ACT && finish && P.act) gelu8(v);
-          if (type == DT_F32) {
-            const int n = ncol + j * 16 + 4 * g16;
-            if (orow < olim && n < P.cols) *(v4f*)(row + n * 4) = v4f{v[0], v[1], v[2], v[3]};
-            if (orow < olim && n + 16 < P.cols) *(v4f*)(row + n * 4 + 64) = v4f{v[4], v[5], v[6], v[7]};
-          } else {
-            unsigned h[4];
-#pragma unroll
-            for (int r = 0; r < 4; r++) h[r] = pack2(v[2 * r], v[2 * r + 1], type);
-            const auto lo = __builtin_amdgcn_permlane16_swap(h[0], h[2], false, false);
-            const auto hi = __builtin_amdgcn_permlane16_swap(h[1], h[3], false, false);
-            const int n = ncol + j * 16 + (g16 & 1) * 16 + (g16 >> 1) * 8;
-            if (orow < olim && n < P.cols) *(v4i*)(row + n * 2) = v4i{(int)lo[0], (int)hi[0], (int)lo[1], (int)hi[1]};
-          }
+        for (int j = 0; j < FN; j++) {
+          const int n = j * 16 + (type == DT_F32 ? 4 * g16 : (g16 & 1) * 16 + (g16 >> 1) * 8);
+          at[j] = (unsigned)((lane & 15) * pitch + n * es) | (n < have ? 0u : kOutOfRange);
         }
-      });
+        for_each<FM>([&](auto I) {  // (the accumulators are registers: their indexes have to be constants)
+          constexpr int i = decltype(I)::value;
+          const unsigned down = (unsigned)(i * 16 * pitch);
+#pragma unroll
+          for (int j = 0; j < FN; j += 2) {
+            float v[8];
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+              v[r] = acc[i][j][r] + bias[j][r];
+              v[r + 4] = acc[i][j + 1][r] + bias[j + 1][r];
+            }
+            if constexpr (decltype(act_of)::value) gelu8(v);
+            if constexpr (type == DT_F32) {
+              __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, v4f{v[0], v[1], v[2], v[3]}), to, at[j] + down, 0, 0);
+              __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, v4f{v[4], v[5], v[6], v[7]}), to, at[j + 1] + down, 0, 0);
+            } else {
+              unsigned h[4];
+#pragma unroll
+              for (int r = 0; r < 4; r++) h[r] = pack2(v[2 * r], v[2 * r + 1], type);
+              const auto lo = __builtin_amdgcn_permlane16_swap(h[0], h[2], false, false);
+              const auto hi = __builtin_amdgcn_permlane16_swap(h[1], h[3], false, false);
+              __builtin_amdgcn_raw_buffer_store_b128(v4u{lo[0], hi[0], lo[1], hi[1]}, to, at[j] + down, 0, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);  // (all pairs at once would want more registers than there are)
+          }
+        });
+      };
+      using F32 = std::integral_constant<int, DT_F32>;
+      using F16 = std::integral_constant<int, DT_F16>;
+      using BF16 = std::integral_constant<int, DT_BF16>;
+      stored = 1;
+      if constexpr (!ACT) {  // 16-bit operands: results of their type, or partial sums
+        if (P.part) emit(F32{}, std::false_type{});
+        else if constexpr (KIND == K_F16) emit(F16{}, std::false_type{});
+        else emit(BF16{}, std::false_type{});
+      } else if (P.act && !P.part) {  // (rows of no expert: GELU keeps the zero)
+        if (type == DT_F32) emit(F32{}, std::true_type{});
+        else if (type == DT_F16) emit(F16{}, std::true_type{});
+        else emit(BF16{}, std::true_type{});
+      } else {
+        if (type == DT_F32) emit(F32{}, std::false_type{});
+        else if (type == DT_F16) emit(F16{}, std::false_type{});
+        else emit(BF16{}, std::false_type{});
+      }
       continue;
     }
     // Rows that allow no 16-byte stores: SR rows at a time go through this wave's own strip of LDS; a lane then holds eight

@@ -78,6 +78,10 @@ struct Job {
   int unit;           // slice (NT / NN) or work unit (TN) the result belongs to
   int s0, s1;         // steps
 };
+struct Sources {
+  const char *p, *q, *ps, *qs;  // operands, 4-bit operands' scales
+  int pn, qn, psn, qsn;         // bytes behind them
+};
 constexpr int kMaxJobs = 64;  // of one workgroup: lane l of every wave holds job l
 
 struct Jobs {
@@ -528,10 +532,12 @@ __device__ __forceinline__ void for_each(F f) { for_each_of(std::make_integer_se
 //     wait for the loads of step i + 1 (issued a whole step ago), barrier
 //     round 1: multiply f1 | read f0 from buffer i + 1 | start loading step i + NB into buffer i
 //
-// Bounds (8 experts, bf16): 16384 x 4096 x 1024 in 149 us = 920 TF/s, the matrix unit 40-60 % busy at the 1.6 GHz the part falls to;
-// 128 x 128 tiles there want 20 TB/s from L2, 256 x 256 ones half of it.  65536 x 1024 x 256 in 63 us: 4 steps per tile, bound by the
-// steps' latency (a lone step takes 0.7-0.9 us whatever its arithmetic) and the results' bytes.  MINW: two workgroups of 128 x 128 per
-// CU cover each other's waits; four (32 x 128) where rows are few.
+// Bounds (8 experts, bf16): 16384 x 4096 x 1024 in 149 us = 920 TF/s, the matrix unit 40-60 % busy at the 1.6 GHz the part falls
+// to; 128 x 128 tiles there want 20 TB/s from L2, 256 x 256 ones half of it.  65536 x 1024 x 256 in 55 us: 4 steps per tile,
+// bound by the steps' latency (a lone step takes 0.7-0.9 us whatever its arithmetic).  Storing nothing saved 4 us there;
+// non-temporal stores save 2 us of a lone 4-bit product and cost the feed-forward 3 %, whose second product then finds less of
+// the first one's result in the caches.  MINW: two workgroups of 128 x 128 per CU cover each other's waits; four (32 x 128)
+// where rows are few.
 template <int KIND, int MODE, int BM, int BN, int WM, int WN, int MINW, int NB = 2>
 __global__ void __launch_bounds__(WM * WN * 64, MINW) tile_kernel(const Params P) {
   constexpr int WAVES = WM * WN, TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
@@ -556,14 +562,7 @@ __global__ void __launch_bounds__(WM * WN * 64, MINW) tile_kernel(const Params P
   jobs.init<MODE == M_TN, BM, BN>(P);
   const int red_steps = MODE == M_TN ? 0 : (int)((P.red + kStepBytes - 1) / kStepBytes);
   const int slice = MODE == M_TN ? 0 : (red_steps + P.splits - 1) / P.splits;
-  auto job_of = [&](int j) {
-    Job w;
-    w.g = __builtin_amdgcn_readlane(jobs.g, j);
-    w.row0 = __builtin_amdgcn_readlane(jobs.row0, j);
-    w.rows = __builtin_amdgcn_readlane(jobs.rows, j);
-    w.col0 = __builtin_amdgcn_readlane(jobs.col0, j);
-    w.prow0 = __builtin_amdgcn_readlane(jobs.prow0, j);
-    w.unit = __builtin_amdgcn_readlane(jobs.unit, j);
+  auto steps_of = [&](Job& w) {
     if constexpr (MODE == M_TN) {
       w.s0 = 0;
       w.s1 = (w.rows + kStepRed - 1) / kStepRed;
@@ -572,6 +571,16 @@ __global__ void __launch_bounds__(WM * WN * 64, MINW) tile_kernel(const Params P
       w.s0 = a < steps ? a : steps;
       w.s1 = w.s0 + slice < steps ? w.s0 + slice : steps;
     }
+  };
+  auto job_of = [&](int j) {
+    Job w;
+    w.g = __builtin_amdgcn_readlane(jobs.g, j);
+    w.row0 = __builtin_amdgcn_readlane(jobs.row0, j);
+    w.rows = __builtin_amdgcn_readlane(jobs.rows, j);
+    w.col0 = __builtin_amdgcn_readlane(jobs.col0, j);
+    w.prow0 = __builtin_amdgcn_readlane(jobs.prow0, j);
+    w.unit = __builtin_amdgcn_readlane(jobs.unit, j);
+    steps_of(w);
     return w;
   };
 
@@ -584,7 +593,54 @@ __global__ void __launch_bounds__(WM * WN * 64, MINW) tile_kernel(const Params P
   const unsigned base = __builtin_amdgcn_readfirstlane((int)lds_address(lds));
   char* const bias_lds = lds + NB * kBuf + WAVES * kStage;
 
+  // Where a job's first step begins in memory, and the bytes from there to the operand's end.  Computed for all jobs at once, lane
+  // j's for job j, and read from there when the loader enters the job: computed anew they are 300 scalar instructions per tile
+  // (4-bit 16384 x 2048 x 512: 47.8 -> 45.5 us; feed-forward of 65536 x 192: 100 -> 94.5).  Not held by 256 x 256 tiles, which
+  // have neither registers for it nor too few steps to hide it, nor by TN's long units (no gain).
+  constexpr bool kHeld = BM < 256 && MODE != M_TN;
+  auto sources_of = [&](const Job& w) {
+    const long k = (long)w.s0 * kStepBytes, r = (long)w.s0 * kStepRed;
+    const int qrows = P.cols - w.col0 < BN ? P.cols - w.col0 : BN;
+    const auto to_int = [](long n) { return n < 0 ? 0 : (int)n; };
+    Sources b{};
+    if constexpr (MODE == M_TN) {
+      b.p = P.p + w.row0 * P.ldp + (long)w.prow0 * 2;
+      b.q = P.q + w.row0 * P.ldq + (long)w.col0 * 2;
+    } else {
+      b.p = P.p + (long)w.row0 * P.ldp + k;
+      b.pn = to_int((long)(w.rows - 1) * P.ldp + (P.red - k));
+      if constexpr (MODE == M_NN) b.q = P.q + w.g * P.strideq + r * P.ldq + (long)w.col0 * 2;
+      else {
+        b.q = P.q + w.g * P.strideq + (long)w.col0 * P.ldq + k;
+        b.qn = to_int((long)(qrows - 1) * P.ldq + (P.red - k));
+      }
+    }
+    if constexpr (KIND == K_MX4) {
+      b.ps = (const char*)P.ps + (long)w.row0 * P.ldps + w.s0 * 8;
+      b.qs = (const char*)P.qs + w.g * P.strideqs + (long)w.col0 * P.ldqs + w.s0 * 8;
+      b.psn = to_int((w.rows - 1) * P.ldps + (P.red - k) / 16);
+      b.qsn = to_int((qrows - 1) * P.ldqs + (P.red - k) / 16);
+    }
+    return b;
+  };
+  Sources held{};
+  if constexpr (kHeld) {
+    Job w{};
+    w.g = jobs.g;
+    w.row0 = jobs.row0;
+    w.rows = jobs.rows;
+    w.col0 = jobs.col0;
+    w.prow0 = jobs.prow0;
+    w.unit = jobs.unit;
+    steps_of(w);
+    held = sources_of(w);
+  }
   int lj = 0, lit = 0, lnum = -1;  // job being loaded, its step, its ordinal among the jobs that load anything
+  auto from_lane = [&](const char* p) {
+    const unsigned long long a = (unsigned long long)p;
+    const unsigned lo = __builtin_amdgcn_readlane((int)(unsigned)a, lj), hi = __builtin_amdgcn_readlane((int)(unsigned)(a >> 32), lj);
+    return (const char*)((unsigned long long)hi << 32 | lo);
+  };
   Job lw{};
   bool more = true;
   int kleft = 0, rleft = 0;  // row operand: bytes, column operand: rows of the reduction that remain
@@ -635,28 +691,26 @@ __global__ void __launch_bounds__(WM * WN * 64, MINW) tile_kernel(const Params P
     }
     lit = lw.s0;
     lnum++;
-    const long k = (long)lit * kStepBytes, r = (long)lit * kStepRed;
-    const int qrows = P.cols - lw.col0 < BN ? P.cols - lw.col0 : BN;
-    kleft = (int)(P.red - k);
-    if constexpr (MODE == M_TN) {
-      rleft = lw.rows - (int)r;
-      lp.start(P.p + (lw.row0 + r) * P.ldp + (long)lw.prow0 * 2, 0);
-      lq.start(P.q + (lw.row0 + r) * P.ldq + (long)lw.col0 * 2, 0);
+    kleft = (int)(P.red - (long)lit * kStepBytes);
+    rleft = MODE == M_TN ? lw.rows - lit * kStepRed : (int)(P.qred - (long)lit * kStepRed);
+    Sources b;
+    if constexpr (kHeld) {
+      b = {from_lane(held.p), from_lane(held.q), from_lane(held.ps), from_lane(held.qs)};
+      b.pn = __builtin_amdgcn_readlane(held.pn, lj);
+      b.qn = __builtin_amdgcn_readlane(held.qn, lj);
+      b.psn = __builtin_amdgcn_readlane(held.psn, lj);
+      b.qsn = __builtin_amdgcn_readlane(held.qsn, lj);
     } else {
-      rleft = (int)(P.qred - r);
-      lp.start(P.p + (long)lw.row0 * P.ldp + k, (long)(lw.rows - 1) * P.ldp + kleft);
-      if constexpr (MODE == M_NN) lq.start(P.q + lw.g * P.strideq + r * P.ldq + (long)lw.col0 * 2, 0);
-      else lq.start(P.q + lw.g * P.strideq + (long)lw.col0 * P.ldq + k, (long)(qrows - 1) * P.ldq + kleft);
+      b = sources_of(lw);
     }
+    lp.start(b.p, b.pn);
+    lq.start(b.q, b.qn);
     if constexpr (KIND == K_MX4) {
-      const unsigned char* psb = P.ps + (long)lw.row0 * P.ldps + lit * 8;
-      const unsigned char* qsb = P.qs + lw.g * P.strideqs + (long)lw.col0 * P.ldqs + lit * 8;
-      const long pbytes = (lw.rows - 1) * P.ldps + kleft / 16, qbytes = (qrows - 1) * P.ldqs + kleft / 16;
       scut = 0;
 #pragma unroll
       for (int c = 0; c < NS; c++) {
         const int i = c * WAVES + wave;  // (pieces behind the last read nothing; their zeros go to padding)
-        sdesc[c] = descriptor(i < BM / 32 ? psb : qsb, i < BM / 32 ? pbytes : i < (BM + BN) / 32 ? qbytes : 0);
+        sdesc[c] = descriptor(i < BM / 32 ? b.ps : b.qs, i < BM / 32 ? b.psn : i < (BM + BN) / 32 ? b.qsn : 0);
       }
     }
     if constexpr (PCOL || QCOL) last_rows();

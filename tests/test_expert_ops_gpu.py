@@ -171,6 +171,21 @@ def test_rows_beyond_32_bit_byte_offsets():
     assert not dx[:-500].any() and torch.equal(y[:1].expand(rows - 500, n), y[:-500])
 
 
+@pytest.mark.parametrize('experts', (63, 64, 65))
+@pytest.mark.parametrize('rows', (90, 3000, 20000))
+def test_as_many_experts_as_lanes(experts, rows):
+    """up to 64 experts the job list is made by one wave's lanes, beyond by a loop; rows: empty experts, whole and cut ones"""
+    off = ragged(experts, rows, experts, head=3, tail=4)
+    x, w, b, dy = _make(experts, rows, experts, 72, 40, torch.bfloat16)
+    _check_all(x, w, b, dy, off, _run(x, w, b, dy, off), torch.bfloat16)
+
+
+def test_more_columns_than_a_tile_addresses():
+    n = (1 << 20) + 8
+    x, w, b, dy = _make(5, 5, 1, n, 32, torch.bfloat16)
+    _check_all(x, w, b, dy, [0, 3], _run(x, w, b, dy, [0, 3]), torch.bfloat16)
+
+
 def test_repeated_calls_other_streams_and_graph_replays_agree():
     from sm3det_amd import expert_ops
     x, w, b, dy = _make(5, 900, 6, 200, 136, torch.bfloat16)

@@ -13,16 +13,22 @@ counts): the host never reads them, so calls are free of synchronisation and can
 * rows of no expert (before ``offsets[0]``, behind ``offsets[-1]``): y and dx are zero there and they enter no gradient.
   Offsets outside [0, rows] are clamped, decreasing ones made monotone.
 * an expert without rows gets zero gradients (never an uninitialised one).
-* first derivatives only: the gradients themselves carry no graph.
+* first derivatives only, backward mode only: the gradients themselves carry no graph, an input with a forward-mode tangent is
+  refused.
 * gradients do not depend on the order in which workgroups run: split reductions are added in a fixed order, no atomics.
 """
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 
 from . import _lib_backbone as LB
 from ._lib import SM3Error, check, lib, require_gpu
 
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def has_tangent(*tensors):
+    """whether forward-mode differentiation (which no_grad() does not end) would have to follow one of the tensors"""
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def check_offsets(offsets, num_groups, device, name):
@@ -147,6 +153,8 @@ def expert_linear(x, w, offsets, b=None):
             raise SM3Error(f'expert_linear: b must be {tuple(w.shape[:2])} of {x.dtype} or float32, got {tuple(b.shape)} of '
                            f'{b.dtype}')
         b = b.contiguous()
+    if has_tangent(x, w, b):
+        raise SM3Error('expert_linear: an input carries a forward-mode tangent; only backward-mode derivatives are implemented')
     offsets = check_offsets(offsets, w.shape[0], x.device, 'expert_linear')
     if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or (b is not None and b.requires_grad)):
         return _ExpertLinear.apply(x, w, offsets, b)

@@ -16,7 +16,7 @@ import torch
 
 from . import _lib_backbone as LB
 from ._lib import SM3Error, check, lib, require_gpu
-from .expert_ops import DTYPES, check_offsets, launch, rows_of
+from .expert_ops import DTYPES, check_offsets, has_tangent, launch, rows_of
 
 ACTS = {None: 0, 'gelu': 1}
 
@@ -94,6 +94,8 @@ def _call(name, device, nbytes, *args):
 def _no_grad(what, *tensors):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise SM3Error(f'{what} is for inference: an input requires a gradient (use torch.no_grad())')
+    if has_tangent(*tensors):
+        raise SM3Error(f'{what} is for inference: an input carries a forward-mode tangent')
 
 
 def quantize(x):
@@ -143,8 +145,7 @@ def _product(what, x, w, offsets, b, act, out_dtype):
         if b.shape != lead or b.dtype not in DTYPES:
             raise SM3Error(f'{what}: b must be {tuple(lead)} of a floating type, got {tuple(b.shape)} of {b.dtype}')
         b = b.contiguous()
-    if torch.is_grad_enabled():
-        _no_grad(what, None if packed else x, b)
+    _no_grad(what, None if packed else x, b)
     if offsets is not None:
         offsets = check_offsets(offsets, groups, device, what)
     M = x.codes.shape[0] if packed else x.shape[0]

@@ -13,8 +13,7 @@ counts): the host never reads them, so calls are free of synchronisation and can
 * rows of no expert (before ``offsets[0]``, behind ``offsets[-1]``): y and dx are zero there and they enter no gradient.
   Offsets outside [0, rows] are clamped, decreasing ones made monotone.
 * an expert without rows gets zero gradients (never an uninitialised one).
-* first derivatives only, backward mode only: the gradients themselves carry no graph, an input with a forward-mode tangent is
-  refused.
+* first derivatives only, backward mode only: differentiating a gradient raises, and so does an input with a forward-mode tangent.
 * gradients do not depend on the order in which workgroups run: split reductions are added in a fixed order, no atomics.
 """
 import torch
@@ -90,51 +89,68 @@ def rows_of(t):
     return t.contiguous(), k
 
 
-def _forward(x, w, offsets, b):
+def _forward(x, ldx, w, offsets, b):
     S, K = x.shape
     E, N, _ = w.shape
     y = torch.empty(S, N, dtype=x.dtype, device=x.device)
-    x, ldx = rows_of(x)
-    w = w.contiguous()
     if S:
         launch('expert_gemm_h16', x.device, LB.NT, DTYPES[x.dtype], y, x, w, S, K, N, ldp=ldx, ldq=K, groups=E, offsets=offsets,
                bias=b, aligned=(x.data_ptr() | w.data_ptr()) & 15 and (x.data_ptr() & 15, w.data_ptr() & 15))
-    return y, x, w
+    return y
+
+
+def _gradients(dy, x, w, offsets, ldx, b_dtype, need):
+    """(dx, dw, db), those that `need` (of x, w, b) asks for"""
+    S, K = x.shape
+    E, N, _ = w.shape
+    dev, dt = x.device, DTYPES[x.dtype]
+    dy, lddy = rows_of(dy)
+    dx = dw = db = None
+    if need[0]:
+        dx = torch.empty(S, K, dtype=x.dtype, device=dev)
+        if S:
+            launch('expert_gemm_h16', dev, LB.NN, dt, dx, dy, w, S, N, K, ldp=lddy, ldq=K, groups=E, offsets=offsets,
+                   aligned=(dy.data_ptr() | w.data_ptr()) & 15 and (dy.data_ptr() & 15, w.data_ptr() & 15))
+    if need[1] or need[2]:
+        # the bias gradient is a by-product of the weight gradient's pass over dy
+        dw = torch.empty(E, N, K, dtype=x.dtype, device=dev)
+        if need[2]:
+            db = torch.empty(E, N, dtype=b_dtype, device=dev)
+        launch('expert_gemm_h16', dev, LB.TN, dt, dw, dy, x, S, 1, K, rows_out=N, ldp=lddy, ldq=ldx, groups=E, offsets=offsets,
+               bias_grad=db, aligned=(dy.data_ptr() | x.data_ptr()) & 15 and (dy.data_ptr() & 15, x.data_ptr() & 15))
+        if not need[1]:
+            dw = None
+    return dx, dw, db
+
+
+class _Gradients(Function):
+    """The gradients where a graph of them is being recorded (create_graph=True): tied to what they were computed from, so that
+    differentiating them raises.  (once_differentiable ties them to dy alone: with a dy that needs no gradient, the part of a loss
+    that depends on dx through w, or on dw through x, would vanish.)"""
+
+    @staticmethod
+    def forward(ctx, dy, x, w, *rest):
+        return _gradients(dy, x, w, *rest)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise SM3Error('expert_linear: second derivatives are not implemented')
 
 
 class _ExpertLinear(Function):
     @staticmethod
-    def forward(ctx, x, w, offsets, b):
-        y, x, w = _forward(x, w, offsets, b)
+    def forward(ctx, x, ldx, w, offsets, b):
         ctx.save_for_backward(x, w, offsets)
-        ctx.b_dtype = None if b is None else b.dtype
-        return y
+        ctx.ldx, ctx.b_dtype = ldx, None if b is None else b.dtype
+        return _forward(x, ldx, w, offsets, b)
 
     @staticmethod
     def backward(ctx, dy):
         x, w, offsets = ctx.saved_tensors
-        S, K = x.shape
-        E, N, _ = w.shape
-        dev, dt = x.device, DTYPES[x.dtype]
-        dy, lddy = rows_of(dy)
-        x, ldx = rows_of(x)
         need = ctx.needs_input_grad
-        dx = dw = db = None
-        if need[0]:
-            dx = torch.empty(S, K, dtype=x.dtype, device=dev)
-            if S:
-                launch('expert_gemm_h16', dev, LB.NN, dt, dx, dy, w, S, N, K, ldp=lddy, ldq=K, groups=E, offsets=offsets,
-                       aligned=(dy.data_ptr() | w.data_ptr()) & 15 and (dy.data_ptr() & 15, w.data_ptr() & 15))
-        if need[1] or need[3]:
-            # the bias gradient is a by-product of the weight gradient's pass over dy
-            dw = torch.empty(E, N, K, dtype=x.dtype, device=dev)
-            if need[3] and ctx.b_dtype is not None:
-                db = torch.empty(E, N, dtype=ctx.b_dtype, device=dev)
-            launch('expert_gemm_h16', dev, LB.TN, dt, dw, dy, x, S, 1, K, rows_out=N, ldp=lddy, ldq=ldx, groups=E, offsets=offsets,
-                   bias_grad=db, aligned=(dy.data_ptr() | x.data_ptr()) & 15 and (dy.data_ptr() & 15, x.data_ptr() & 15))
-            if not need[1]:
-                dw = None
-        return dx, dw, None, db
+        f = _Gradients.apply if torch.is_grad_enabled() else _gradients
+        dx, dw, db = f(dy, x, w, offsets, ctx.ldx, ctx.b_dtype, (need[0], need[2], need[4]))
+        return dx, None, dw, None, db
 
 
 def expert_linear(x, w, offsets, b=None):
@@ -156,6 +172,8 @@ def expert_linear(x, w, offsets, b=None):
     if has_tangent(x, w, b):
         raise SM3Error('expert_linear: an input carries a forward-mode tangent; only backward-mode derivatives are implemented')
     offsets = check_offsets(offsets, w.shape[0], x.device, 'expert_linear')
+    # (copies are made here, where autograd sees them: what it saves are then the caller's tensors or lead to them)
+    (x, ldx), w = rows_of(x), w.contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or (b is not None and b.requires_grad)):
-        return _ExpertLinear.apply(x, w, offsets, b)
-    return _forward(x, w, offsets, b)[0]
+        return _ExpertLinear.apply(x, ldx, w, offsets, b)
+    return _forward(x, ldx, w, offsets, b)

@@ -78,3 +78,47 @@ def test_forward_mode_derivatives_of_the_4_bit_calls_are_refused(monkeypatch, gr
                      lambda f: mx4.expert_linear(x, we, off, f(be))):
             call(lambda t: t)
             _refused(lambda: call(d))
+
+
+SECOND = [  # what needs a gradient of (x, w, b, dy); strided inputs are copied on their way in
+    (which, strided) for which in ((0, 1), (1, 2), (0, 1, 2), (0,), (1,), (0, 1, 2, 3)) for strided in (False, True)]
+
+
+@pytest.mark.parametrize('which,strided', SECOND, ids=str)
+def test_a_second_derivative_is_refused_not_dropped(ops, which, strided):
+    """loss = y . dy + |first gradient|^2: whatever input of the second term the caller differentiates with respect to, the
+    call raises -- also where the gradient that came in carries no graph itself, and where the other input alone does"""
+    x, w, b, dy, off = _inputs(torch.float16)
+    if strided:  # unit stride along neither dimension
+        x = torch.stack([x, x], -1)[..., 0]
+        w = torch.stack([w, w], -1)[..., 0]
+    leaves = [t.clone(memory_format=torch.preserve_format).requires_grad_(i in which) if not strided else t.requires_grad_(i in which)
+              for i, t in enumerate((x, w, b, dy))]
+    x, w, b, dy = leaves
+    asked = [t for t in leaves[:3] if t.requires_grad]
+    y = ops.expert_linear(x, w, off, b)
+    firsts = torch.autograd.grad(y, asked, dy, create_graph=True)
+    # dx depends on (dy, w), dw on (dy, x), db on dy
+    depends = {id(x): [w, dy], id(w): [x, dy], id(b): [dy]}
+    for leaf, first in zip(asked, firsts):
+        for other in depends[id(leaf)]:
+            if other.requires_grad:
+                mixed = (y * dy.detach()).double().sum() + first.double().square().sum()
+                _refused(lambda: torch.autograd.grad(mixed, other, retain_graph=True, allow_unused=True))
+
+
+def test_first_derivatives_are_the_formulas_with_and_without_a_graph(ops):
+    x, w, b, dy, off = _inputs(torch.float16)
+    for graph in (False, True):
+        for leaves in ([t.clone().requires_grad_() for t in (x, w, b)],
+                       [torch.stack([t, t], -1)[..., 0].requires_grad_() for t in (x, w, b)]):
+            y = ops.expert_linear(leaves[0], leaves[1], off, leaves[2])
+            dx, dw, db = torch.autograd.grad(y, leaves, dy, create_graph=graph)
+            for g, (p, q) in enumerate(((1, 4), (4, 8))):
+                assert torch.equal(y[p:q].double(), x[p:q].double() @ w[g].double().t() + b[g].double())
+                assert torch.equal(dx[p:q].double(), dy[p:q].double() @ w[g].double())
+                assert torch.equal(dw[g].double(), dy[p:q].double().t() @ x[p:q].double())
+                assert torch.equal(db[g].double(), dy[p:q].double().sum(0))
+            assert not y[:1].any() and not y[8:].any() and not dx[:1].any() and not dx[8:].any()
+            for leaf, got in zip(leaves, (dx, dw, db)):
+                assert got.shape == leaf.shape and got.dtype == leaf.dtype

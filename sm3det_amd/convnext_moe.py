@@ -139,15 +139,32 @@ class MoE_layer(nn.Module):
         self.last_importance_load = None  # device fp32 (2E): [importance | load] of the last forward
         self.last_top_idx = None  # device int32 (T, min(k+1,E)): the routing of the last forward, best first
 
-    _mx4 = None  # packed 4-bit (w1, w2) of mx4.quantize_experts; gone when the weights may change or move
+    _mx4 = None  # the 4-bit experts (mx4.PackedExperts) of mx4.quantize_experts
 
     def experts(self):
         """what takes the place of the expert FFNs in this forward: None, or the 4-bit experts (evaluation only)"""
-        if self._mx4 is None:
+        packed = self._mx4
+        if packed is None or not packed.made_from(self):
             return None
-        from . import mx4
-        (w1, w2), b1, b2 = self._mx4, self.b1, self.b2
-        return lambda xslot, offsets: mx4.expert_ffn(xslot, w1, b1.detach(), w2, b2.detach(), offsets)
+        if not packed.followable():
+            from . import mx4
+            packed = mx4.PackedExperts(self)
+        elif self.w1.is_cuda and torch.cuda.is_current_stream_capturing():
+            held = self.__dict__.setdefault('_mx4_captured', [])  # the graph reads them in every replay
+            if not any(h is packed for h in held):
+                held.append(packed)
+        return packed.ffn
+
+    def __getstate__(self):  # copies and pickles: a snapshot that is of use goes along, what graphs of this layer read does not
+        state = {k: v for k, v in self.__dict__.items() if k != '_mx4_captured'}
+        if self._mx4 is not None and not self._mx4.made_from(self):
+            state['_mx4'] = None
+        return state
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        if self._mx4 is not None:
+            self._mx4.stamp(self)
 
     def train(self, mode=True):
         if mode:

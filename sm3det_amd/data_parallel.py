@@ -195,6 +195,7 @@ class BucketedGradReducer:
                         todo.append(t)
             for t in todo:
                 dist.broadcast(t.data, src=src, group=self.group)
+                torch.autograd.graph.increment_version(t)  # (`.data` has a version of its own: caches made from t look at t's)
 
     def remove_hooks(self):
         for h in self._hooks:

@@ -184,17 +184,58 @@ def expert_ffn(x, w1, b1, w2, b2, offsets):
     return expert_linear(h, w2, offsets, b2, out_dtype=torch.float32)
 
 
+class PackedExperts:
+    """The experts of one MoE layer as the 4-bit products read them -- packed weights, a copy of the biases -- and the state of the
+    four parameters they were made from, so that they are never used for other values."""
+
+    def __init__(self, layer):
+        self.w1, self.w2 = quantize(layer.w1.detach()), quantize(layer.w2.detach())
+        self.b1, self.b2 = layer.b1.detach().clone(), layer.b2.detach().clone()
+        self.stamp(layer)
+
+    def stamp(self, layer):
+        """these are `layer`'s parameters as they are now"""
+        self.states = [self._state(p) for p in (layer.w1, layer.b1, layer.w2, layer.b2)]
+
+    @staticmethod
+    def _state(p):
+        # (an optimizer that writes by address does not move the version: it counts its steps, MultiTensorAdamW._writer)
+        return p, p.data_ptr(), None if p.is_inference() else p._version, [(w, w.steps) for w in getattr(p, '_sm3_writers', ())]
+
+    def made_from(self, layer):
+        """whether nothing the host sees has changed the parameters since"""
+        return all(p is s[0] and self._state(p)[1:] == s[1:] for p, s in zip((layer.w1, layer.b1, layer.w2, layer.b2), self.states))
+
+    def followable(self):
+        """False: writes may come that the host does not see -- an optimizer step inside a captured graph, parameters that keep no
+        version"""
+        return not any(version is None or any(w.captured for w, _ in writers) for _, _, version, writers in self.states)
+
+    def ffn(self, xslot, offsets):
+        return expert_ffn(xslot, self.w1, self.b1, self.w2, self.b2, offsets)
+
+    def __getstate__(self):  # (a copy of the layer has parameters of its own: MoE_layer.__setstate__ stamps)
+        return {k: v for k, v in self.__dict__.items() if k != 'states'}
+
+
 def quantize_experts(module):
     """Pack the experts of every MoE layer inside `module` (a backbone or a detector in evaluation mode): its forward under
     ``torch.no_grad()`` then runs them on the 4-bit products -- router, combine, dense blocks and everything else as before.
-    The packed weights are a snapshot: ``train()``, ``load_state_dict()`` and moving the module drop them.  -> layers packed."""
+    -> layers packed.
+
+    The packed weights (and the biases next to them) are a snapshot.  ``train()``, ``load_state_dict()`` and moving the module drop
+    them; after any other change of w1, b1, w2 or b2 -- a torch operation in place, a step of ``MultiTensorAdamW``, a broadcast, other
+    parameters in their place -- the layer runs its full-precision experts until it is packed again.  Where a captured
+    optimizer step writes the parameters, whose replays nobody announces, every forward packs them anew.  Not seen: values
+    written past autograd's version counter (``p.data.copy_()``, a foreign kernel); call this again after those.
+    A graph captured from such a forward replays the snapshot, which the layer keeps allocated for it: capture again after a change."""
     from .convnext_moe import MoE_layer
     layers = [m for m in module.modules() if isinstance(m, MoE_layer)]
     for m in layers:
         if m.training:
             raise SM3Error('mx4.quantize_experts: call module.eval() first (4-bit experts are for inference)')
-    for m in layers:
-        m._mx4 = (quantize(m.w1.detach()), quantize(m.w2.detach()))
+    for m, packed in [(m, PackedExperts(m)) for m in layers]:
+        m._mx4 = packed
     return len(layers)
 
 

@@ -24,6 +24,13 @@ from . import _lib
 from . import _lib_backbone as LB
 
 
+class _Writer:
+    """Hung on the parameters that an optimizer writes by address, which moves no version counter: what was made from a parameter
+    (mx4.PackedExperts) looks here whether it is still of use."""
+    steps = 0
+    captured = False  # a step went into a graph: its replays count nowhere
+
+
 class MultiTensorAdamW(torch.optim.Optimizer):
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_grad_norm=None,
                  loss_scale=None):
@@ -36,6 +43,7 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         super().__init__(params, defaults)
         self.max_grad_norm = float(max_grad_norm) if max_grad_norm else 0.0
         self._built = False
+        self._writer = _Writer()
         self._n_steps_host = 0  # steps taken (host-side count; only used to flag late-joining parameters)
         self._last_hyper = None
         self._scaler = None
@@ -156,6 +164,9 @@ class MultiTensorAdamW(torch.optim.Optimizer):
             raise _lib.SM3Error('MultiTensorAdamW: no parameter has a gradient')
         dev = ps[0][1].device
         self._params = ps
+        for _, p in ps:
+            if self._writer not in getattr(p, '_sm3_writers', ()):
+                p._sm3_writers = (*getattr(p, '_sm3_writers', ()), self._writer)
         chunk = _lib.lib().sm3_optim_chunk_elems()
         tab = []
         for ti, (_, p) in enumerate(ps):
@@ -272,6 +283,8 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         elif not torch.cuda.is_current_stream_capturing():
             self.refresh_grad_pointers()
             self.update_hyperparams()
+        self._writer.steps += 1
+        self._writer.captured |= torch.cuda.is_current_stream_capturing()
         g0 = self.param_groups[0]
         b1, b2 = g0['betas']
         self._n_steps_host += 1

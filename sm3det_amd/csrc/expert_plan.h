@@ -23,6 +23,9 @@ struct Plan {
   size_t total() const { return part_bytes + bsum_bytes + p_bytes + p_scale_bytes + q_bytes; }
 };
 
+// elements of an operand's row (16 bits), and between rows: byte offsets inside a tile of up to 256 rows have 31 bits
+constexpr long kMostElements = 1L << 22;
+
 // jobs are counted in 31 bits
 inline bool fits(const Plan& p) { return (double)p.per_xcd * kNumXCD < 2.0e9 && (double)p.units < 2.0e9; }
 
@@ -36,10 +39,8 @@ inline int check_desc(const sm3_expert_desc* d, bool mx4) {
   if (d->mode == SM3_GEMM_TN ? d->rows_out < 1 || d->bias || d->act : d->bias_grad != nullptr) return SM3_ERR_INVALID_ARG;
   const bool reads = d->rows > 0;  // (a weight gradient over no rows writes zeros)
   if (!d->out || (reads && (!d->p || !d->q))) return SM3_ERR_INVALID_ARG;
-  // 32-bit offsets inside a tile: up to 256 rows of either operand
-  const long most = 1L << 22;
   const long prow = d->mode == SM3_GEMM_TN ? d->rows_out : d->red, qrow = d->mode == SM3_GEMM_NT ? d->red : d->cols;
-  if (prow > most || qrow > most || d->cols > 1 << 30) return SM3_ERR_UNSUPPORTED;
+  if (prow > kMostElements || qrow > kMostElements || d->cols > 1 << 30) return SM3_ERR_UNSUPPORTED;
   if (mx4) {
     if (!d->q_scales || (uintptr_t)d->q % 16 || (uintptr_t)d->q_scales % 4) return SM3_ERR_INVALID_ARG;
     if (d->p_scales) {
@@ -57,7 +58,7 @@ inline int check_desc(const sm3_expert_desc* d, bool mx4) {
 
 // rows the tile kernel can read as they are
 inline bool readable(const void* p, long ld, long row) {
-  return (uintptr_t)p % 16 == 0 && ld % 8 == 0 && row % 8 == 0 && ld <= 1L << 22;
+  return (uintptr_t)p % 16 == 0 && ld % 8 == 0 && row % 8 == 0 && ld <= kMostElements;
 }
 
 inline Plan plan_tiles(const sm3_expert_desc* d, bool mx4) {
@@ -97,7 +98,9 @@ inline Plan plan_tiles(const sm3_expert_desc* d, bool mx4) {
   const long red_steps = ((mx4 ? (d->red + 127) / 128 * 64 : d->red * 2L) + kStepBytes - 1) / kStepBytes;
   const long some = d->offsets ? (d->num_groups < d->rows ? d->num_groups : d->rows) / 2 : 0;  // half a tile is lost per expert
   const long expected = ((d->rows + 255) / 256 + some) * ((d->cols + 255L) / 256);
-  if (!mx4 && expected / kNumCU * red_steps >= 48 && red_steps >= 8 && d->cols % 256 == 0) {
+  // (256 rows of the longest reduction would be 2^31 bytes, one more than a tile's range counts: 128 x 128 tiles)
+  const bool countable = d->red <= kMostElements - 8;
+  if (!mx4 && countable && expected / kNumCU * red_steps >= 48 && red_steps >= 8 && d->cols % 256 == 0) {
     p.coarse = true;
     p.bm = p.bn = 256;
   }

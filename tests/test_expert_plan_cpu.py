@@ -97,3 +97,27 @@ def test_the_4_bit_sizes(plan, name):
     if least > 1:
         tiles = _row_tiles(rows, offsets or [0, rows], p['bm']) * ((n + 127) // 128)
         assert _per_workgroup(tiles, 3 if p['bm'] == 32 else 2) > least - 1
+
+
+@pytest.mark.parametrize('red', (1 << 12, (1 << 22) - 64, (1 << 22) - 8, (1 << 22) - 7, (1 << 22) - 1, 1 << 22))
+@pytest.mark.parametrize('ld', (0, 1 << 22))
+def test_the_bytes_of_a_tiles_rows_stay_below_2_to_the_31(plan, red, ld):
+    """rows of the reduction's length, padded to 8 where the kernel copies them; a part of a wider matrix where ld says so"""
+    for mode in (NT, NN):
+        for rows in (1, 300, 4096, 70000):
+            n, k = (4096, red) if mode == NT else (red, 4096)
+            kw = dict(ldp=ld) if ld else {}
+            if ld and mode == NT:
+                kw.update(ldq=ld)
+            p = plan(mode, rows, 1, n, k, **kw)
+            row = (red + 7) // 8 * 8
+            pitch = max(ld, row) if not p['copies_p'] else row
+            assert ((p['bm'] - 1) * pitch + row) * 2 < 1 << 31, (mode, rows, p)
+            assert mode == NN or ((p['bn'] - 1) * pitch + row) * 2 < 1 << 31, (mode, rows, p)
+            if rows >= 4096 and red < (1 << 22) - 7:
+                assert p['coarse']
+
+
+def test_longer_reductions_are_refused(plan):
+    for mode, n, k in ((NT, 4096, (1 << 22) + 1), (NN, (1 << 22) + 1, 4096), (TN, 4096, (1 << 22) + 1), (TN, (1 << 22) + 1, 4096)):
+        assert plan(mode, 4096, 1, n, k) == -4

@@ -717,7 +717,8 @@ __global__ void __launch_bounds__(WM * WN * 64, MINW) tile_kernel(const Params P
     if constexpr (!PCOL) { if (kleft < kStepBytes) last_bytes(); }
     if constexpr (MODE != M_TN) {
       if (P.bias_lds && wave * 256 < BN * bes) {
-        bdesc = descriptor((const char*)P.bias + ((long)lw.g * P.cols + lw.col0) * bes, (long)(P.cols - lw.col0) * bes);
+        const int bcols = P.cols - lw.col0 < BN ? P.cols - lw.col0 : BN;  // (all of a long row would not be counted in 32 bits)
+        bdesc = descriptor((const char*)P.bias + ((long)lw.g * P.cols + lw.col0) * bes, bcols * bes);
         bias_to = base + (unsigned)(bias_lds - lds) + (lnum & 3) * (BN * 4) + wave * 256;
       }
     }

@@ -131,3 +131,22 @@ def test_the_longest_reductions(red):
     torch.cuda.empty_cache()
     ref = X @ W.t()
     assert_within(y, ref, bound(ref, X.abs() @ W.abs().t(), 3 * 64, torch.bfloat16))  # (added zeros are exact)
+
+
+@pytest.mark.parametrize('bias', (torch.float32, torch.bfloat16))
+def test_a_bias_row_of_2_to_the_32_bytes(bias):
+    from sm3det_amd import expert_ops
+    n = 1 << 30
+    w = torch.zeros(1, n, 8, dtype=torch.bfloat16, device='cuda')
+    b = torch.ones(1, n, dtype=bias, device='cuda')
+    some = torch.cat([torch.arange(300), n // 2 + torch.arange(300), n - 300 + torch.arange(300)]).cuda()
+    w[0, some], b[0, some] = _randn(1, 900, 8, dtype=w.dtype), _randn(2, 900, dtype=bias)
+    x = _randn(3, 2, 8, dtype=w.dtype)
+    y = expert_ops.expert_linear(x, w, torch.tensor([0, 2], dtype=torch.int32, device='cuda'), b)
+    W, B = w[0, some].double(), b[0, some].double()
+    ref = x.double() @ W.t() + B
+    assert_within(y[:, some], ref, bound(ref, x.double().abs() @ W.abs().t() + B.abs(), 8, torch.bfloat16))
+    rest = int((y == 1).sum()) - int((y[:, some] == 1).sum())
+    del w, b, y
+    torch.cuda.empty_cache()
+    assert rest == 2 * (n - 900)

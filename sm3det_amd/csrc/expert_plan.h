@@ -295,7 +295,7 @@ inline Params params_of(const sm3_expert_desc* d, const Plan& pl, bool mx4, cons
   P.unit_rows = pl.unit_rows;
   P.part = ws.part;
   const long bes = d->bias_type == SM3_DT_F32 ? 4 : 2;
-  P.bias_lds = d->bias && (uintptr_t)d->bias % 4 == 0 && d->cols * bes % 4 == 0;
+  P.bias_lds = d->bias && (uintptr_t)d->bias % 4 == 0 && d->cols * bes % 4 == 0 && d->cols * bes < 1L << 32;
   P.wide = P.part ? d->cols % 4 == 0 : d->cols % (d->out_type == SM3_DT_F32 ? 4 : 8) == 0 && (uintptr_t)d->out % 16 == 0;
   if (d->cols > 1 << 20) P.wide = 0;  // (those stores address a tile's 128 rows with 31 bits)
   P.bsum = ws.bsum;

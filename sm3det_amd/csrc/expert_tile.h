@@ -52,7 +52,7 @@ struct Params {
   int rows_out, cols;             // TN: output rows of one expert; output columns
   int out_type, bias_type, act;
   int wide;                       // result rows allow 16-byte stores
-  int bias_lds;                   // bias rows may be loaded as 4-byte words
+  int bias_lds;                   // bias rows may be loaded as 4-byte words and their bytes are counted in 32 bits
   const void* bias;               // (G, cols) or null
   void* db;                       // TN: column sums of p per expert (G, rows_out) of bias_type, or null;
   float* bsum;                    // where units are parts of experts: per unit (units, rows_out) fp32
@@ -717,8 +717,7 @@ __global__ void __launch_bounds__(WM * WN * 64, MINW) tile_kernel(const Params P
     if constexpr (!PCOL) { if (kleft < kStepBytes) last_bytes(); }
     if constexpr (MODE != M_TN) {
       if (P.bias_lds && wave * 256 < BN * bes) {
-        const int bcols = P.cols - lw.col0 < BN ? P.cols - lw.col0 : BN;  // (all of a long row would not be counted in 32 bits)
-        bdesc = descriptor((const char*)P.bias + ((long)lw.g * P.cols + lw.col0) * bes, bcols * bes);
+        bdesc = descriptor((const char*)P.bias + ((long)lw.g * P.cols + lw.col0) * bes, (long)(P.cols - lw.col0) * bes);
         bias_to = base + (unsigned)(bias_lds - lds) + (lnum & 3) * (BN * 4) + wave * 256;
       }
     }

@@ -7,11 +7,18 @@ using namespace sm3x;
 
 namespace {
 
-// A handful of rows per expert, not yet quantised: one launch without a workspace (mx4_few.hip).  Up to 16 rows an expert's
-// rows are one tile there; with more the weights would be read again for every 16 rows.
+// A handful of rows, not yet quantised: one launch without a workspace (mx4_few.hip).  Up to 16 rows an expert's rows are one tile
+// there.  Every 16 columns of every tile quantise their rows again, so its time grows with tiles x columns x reduction (the tiles as
+// the host can bound them: the rows' spread over the experts is known to the device alone), while quantisation, tile kernel and their
+// host side cost about 13 us from the start.  Measured on 2 to 64 experts, 64 x 64 to 4096 x 1024, bf16 / fp32 rows, us per call
+// back to back, here against there: up to 1 M of that product 9 against 13.5; 8 experts, 64 rows, 4096 x 1024 (3.1 M) 12.6 / 17.3
+// against 13.8 / 15.2; 16 experts, 256 rows, 2048 x 512 (2.1 M) 14.4 / 23.8 against 13.5 / 15.7; 64 experts, 1000 rows, 4096 x
+// 1024 (33 M) 102 / 188 against 30 / 31.
 bool few(const sm3_expert_desc* d) {
   const long experts = d->num_groups < d->rows ? d->num_groups : d->rows;
-  return !d->p_scales && d->rows <= 16 * experts && row_tiles(d->rows, d->num_groups, d->offsets != nullptr, 16) < 65536;
+  if (d->p_scales || d->rows > 16 * experts || row_tiles(d->rows, d->num_groups, d->offsets != nullptr, 16) >= 65536) return false;
+  const double work = (double)(d->rows / 16 + experts) * ((d->cols + 15) / 16) * ((d->red + 127) / 128 * 128);
+  return d->rows <= 16 || work <= (d->type == SM3_DT_F32 ? 2.5e6 : 3.4e6);
 }
 
 }  // namespace

@@ -58,3 +58,14 @@ MX4 = {
     'sliced_dense': (200, None, 388, 2100, 1, 2),
     'sliced_rows_of_16_bytes': (700, offsets_of(3, [600, 90]), 256, 2048, 1, 2),
 }
+
+# 4-bit products of few rows per expert: name -> (rows, offsets, n, k, one launch for bf16, for float32 rows)
+FEW = {
+    'a_token': (1, offsets_of(0, [0, 1, 0]), 2048, 512, True, True),
+    'sixteen_rows': (16, offsets_of(0, [1] * 7 + [0, 9]), 4096, 1024, True, True),
+    'few_columns': (1000, offsets_of(0, [0, 30, 1, 16, 17] * 12 + [0, 200, 20, 0]), 64, 64, True, True),
+    'by_the_type': (64, offsets_of(0, [0, 17, 1, 16, 9, 13, 8, 0]), 4096, 1024, True, False),
+    'many_tiles': (256, offsets_of(0, [0, 17, 1, 16, 9, 13, 8, 0, 60, 20, 20, 33, 31, 1, 0, 27]), 2048, 512, True, True),
+    'one_experts_rows': (1000, offsets_of(0, [0] * 5 + [1000] + [0] * 58), 2048, 512, False, False),
+    'every_experts_rows': (1000, offsets_of(3, [0, 30, 1, 16, 17] * 12 + [0, 200, 20, 0]), 2048, 512, False, False),
+}

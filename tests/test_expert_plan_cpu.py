@@ -5,7 +5,7 @@ import subprocess
 
 import pytest
 
-from tests.expert_shapes import COARSE, MX4, SEVERAL, WEIGHT
+from tests.expert_shapes import COARSE, FEW, MX4, SEVERAL, WEIGHT
 
 SOURCE = """
 #include "expert_plan.h"
@@ -121,3 +121,15 @@ def test_the_bytes_of_a_tiles_rows_stay_below_2_to_the_31(plan, red, ld):
 def test_longer_reductions_are_refused(plan):
     for mode, n, k in ((NT, 4096, (1 << 22) + 1), (NN, (1 << 22) + 1, 4096), (TN, 4096, (1 << 22) + 1), (TN, (1 << 22) + 1, 4096)):
         assert plan(mode, 4096, 1, n, k) == -4
+
+
+@pytest.mark.parametrize('name', FEW)
+def test_few_rows_run_in_one_launch_while_that_is_the_faster_way(name):
+    """(one launch: no workspace) -- by the rows, the experts and the sizes of the product, not by the mean load alone"""
+    from sm3det_amd import _lib
+    from sm3det_amd._lib_backbone import EXPERT_DESC
+    rows, offsets, n, k, bf16, fp32 = FEW[name]
+    a = 1 << 20
+    for dtype, one in ((0, fp32), (1, bf16), (2, bf16)):
+        desc = EXPERT_DESC.pack(0, dtype, dtype, 0, 0, len(offsets) - 1, k, n, 0, 0, rows, k, 0, a, a, 0, a, a, 0, 0, a)
+        assert (_lib.lib().sm3_mx4_gemm_workspace_bytes(desc) == 0) == one, dtype

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from tests.expert_common import HALF_STEP, assert_within, bound, spans
-from tests.expert_shapes import COARSE, MX4, SEVERAL, WEIGHT
+from tests.expert_shapes import COARSE, FEW, MX4, SEVERAL, WEIGHT
 from tests.test_expert_ops_gpu import _check_all, _run
 from tests.test_mx4_gpu import _check, _values
 
@@ -67,10 +67,10 @@ def test_nan_rows_of_no_expert_and_one_experts_infinities_stay_out(name):
 @pytest.mark.parametrize('act', (None, 'gelu'))
 @pytest.mark.parametrize('bias', (False, True))
 @pytest.mark.parametrize('dtype', DT)
-@pytest.mark.parametrize('name', MX4)
+@pytest.mark.parametrize('name', (*MX4, *FEW))
 def test_4_bit_products(name, dtype, act, bias):
     from sm3det_amd import mx4
-    rows, offsets, n, k = MX4[name][:4]
+    rows, offsets, n, k = {**MX4, **FEW}[name][:4]
     dt, e = DT[dtype], len(offsets) - 1 if offsets else 1
     x = _randn(1, rows, k, dtype=dt)
     w = mx4.quantize(_randn(2, e, n, k, dtype=torch.float32, scale=k ** -0.5))
@@ -83,7 +83,7 @@ def test_4_bit_products(name, dtype, act, bias):
     else:
         off = torch.tensor(offsets, dtype=torch.int32, device='cuda')
         y, packed = (mx4.expert_linear(t, w, off, b, act=act, out_dtype=dt) for t in (x, xq))
-    if rows > 16 * e:  # (few rows per expert have a kernel of their own unless they come packed)
+    if name in MX4:  # (few rows per expert have a kernel of their own unless they come packed)
         assert torch.equal(y, packed)
     left = torch.ones(rows, dtype=torch.bool, device='cuda')
     for g, (p, q) in enumerate(spans(offsets or [0, rows], rows)):

@@ -120,6 +120,8 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const unsigned* __restr
   }
 }
 
+constexpr int kMaxRow = 0x7fffff80;  // (padded, its elements are counted in 31 bits)
+
 inline unsigned blocks_for(long total) {
   const long b = (total + 255) / 256;
   return (unsigned)(b > 16384 ? 16384 : b);
@@ -132,6 +134,7 @@ extern "C" {
 int sm3_mx4_quantize(const void* x, int type, long rows, int k, long ld, uint8_t* codes, uint8_t* scales,
                      sm3_stream_t stream) {
   if (rows < 0 || k < 1 || ld < k || type < 0 || type > SM3_DT_BF16) return SM3_ERR_INVALID_ARG;
+  if (k > kMaxRow) return SM3_ERR_UNSUPPORTED;
   if (rows == 0) return SM3_OK;
   if (!x || !codes || !scales || ((uintptr_t)codes & 3)) return SM3_ERR_INVALID_ARG;
   const unsigned octets = (unsigned)((k + 127) / 128 * 16);
@@ -152,6 +155,7 @@ int sm3_mx4_quantize(const void* x, int type, long rows, int k, long ld, uint8_t
 int sm3_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, long rows, int k, void* y, int type,
                        sm3_stream_t stream) {
   if (rows < 0 || k < 1 || type < 0 || type > SM3_DT_BF16) return SM3_ERR_INVALID_ARG;
+  if (k > kMaxRow) return SM3_ERR_UNSUPPORTED;
   if (rows == 0) return SM3_OK;
   if (!y || !codes || !scales || ((uintptr_t)codes & 3)) return SM3_ERR_INVALID_ARG;
   const unsigned octets = (unsigned)((k + 127) / 128 * 16);

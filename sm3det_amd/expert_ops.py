@@ -8,8 +8,8 @@ block of ``backbone_ops.moe_block``.  ``offsets`` are what ``sm3_moe_plan`` leav
 counts): the host never reads them, so calls are free of synchronisation and can be captured into a HIP graph.
 
 * types: x, w both bfloat16 or both float16, fp32 accumulation, results rounded once; b of x's type or float32.
-* any sizes and row strides (rows of a length that is no multiple of 8, or not 16-byte aligned, are copied into padded rows of
-  the workspace first).
+* any sizes and row strides, rows and reductions of up to 2^22 elements (rows of a length that is no multiple of 8, or not 16-byte
+  aligned, are copied into padded rows of the workspace first).
 * rows of no expert (before ``offsets[0]``, behind ``offsets[-1]``): y and dx are zero there and they enter no gradient.
   Offsets outside [0, rows] are clamped, decreasing ones made monotone.
 * an expert without rows gets zero gradients (never an uninitialised one).
@@ -54,11 +54,15 @@ def launch(fn, device, mode, dtype, out, p, q, rows, red, cols, *, rows_out=0, l
     L = lib()
     b = bias if bias is not None else bias_grad
     out_type = DTYPES[out.dtype]
-    desc = LB.EXPERT_DESC.pack(
-        mode, dtype, out_type, 0 if b is None else DTYPES[b.dtype], act, groups, red, cols, rows_out, 0, rows, ldp, ldq,
-        p.data_ptr(), q.data_ptr(), 0 if p_scales is None else p_scales.data_ptr(), 0 if q_scales is None else q_scales.data_ptr(),
-        0 if offsets is None else offsets.data_ptr(), 0 if bias is None else bias.data_ptr(),
-        0 if bias_grad is None else bias_grad.data_ptr(), out.data_ptr())
+    try:
+        desc = LB.EXPERT_DESC.pack(
+            mode, dtype, out_type, 0 if b is None else DTYPES[b.dtype], act, groups, red, cols, rows_out, 0, rows, ldp, ldq,
+            p.data_ptr(), q.data_ptr(), 0 if p_scales is None else p_scales.data_ptr(), 0 if q_scales is None else q_scales.data_ptr(),
+            0 if offsets is None else offsets.data_ptr(), 0 if bias is None else bias.data_ptr(),
+            0 if bias_grad is None else bias_grad.data_ptr(), out.data_ptr())
+    except LB.struct.error:
+        raise SM3Error(f'{fn}: sizes are counted in 31 bits: reduction {red}, columns {cols}, rows of the result {rows_out}, '
+                       f'experts {groups}') from None
     key = (fn, mode, dtype, out_type, groups, red, cols, rows_out, rows, ldp, ldq, offsets is None, bias_grad is None,
            p_scales is None, aligned)
     need = _NEED.get(key)

@@ -19,6 +19,7 @@ from ._lib import SM3Error, check, lib, require_gpu
 from .expert_ops import DTYPES, check_offsets, has_tangent, launch, rows_of
 
 ACTS = {None: 0, 'gelu': 1}
+MAX_K = 0x7fffff80  # elements of a row: padded, they are counted in 31 bits
 
 
 def padded(k):
@@ -36,6 +37,8 @@ class Mx4Tensor:
         kp = padded(k) if k > 0 else 0
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.device != scales.device:
             raise SM3Error('Mx4Tensor: codes and scales must be uint8 tensors on one device')
+        if k > MAX_K:
+            raise SM3Error(f'Mx4Tensor: rows of at most {MAX_K} elements, got {k}')
         if kp == 0 or len(cs) < 2 or cs[:-1] != ss[:-1] or cs[-1] * 2 != kp or ss[-1] * 32 != kp:
             raise SM3Error(f'Mx4Tensor: rows of {k} elements need codes (..., {kp // 2}) and scales (..., {kp // 32}), got '
                            f'{tuple(cs)} and {tuple(ss)}')
@@ -105,6 +108,8 @@ def quantize(x):
     if x.dtype not in DTYPES or x.dim() < 2 or x.shape[-1] < 1:
         raise SM3Error(f'mx4.quantize: (..., K) float32, float16 or bfloat16 rows expected, got {tuple(x.shape)} of {x.dtype}')
     K = x.shape[-1]
+    if K > MAX_K:
+        raise SM3Error(f'mx4.quantize: rows of at most {MAX_K} elements, got {K}')
     x, ld = rows_of(x) if x.dim() == 2 else (x.contiguous(), K)
     kp = (K + 127) // 128 * 128
     codes = torch.empty(*x.shape[:-1], kp // 2, dtype=torch.uint8, device=x.device)

@@ -146,10 +146,10 @@ class MoE_layer(nn.Module):
         packed = self._mx4
         if packed is None or not packed.made_from(self):
             return None
-        if not packed.followable():
+        if not packed.followable:
             from . import mx4
             packed = mx4.PackedExperts(self)
-        elif self.w1.is_cuda and torch.cuda.is_current_stream_capturing():
+        elif packed.b1.is_cuda and torch.cuda.is_current_stream_capturing():
             held = self.__dict__.setdefault('_mx4_captured', [])  # the graph reads them in every replay
             if not any(h is packed for h in held):
                 held.append(packed)

@@ -91,10 +91,13 @@ inline Plan plan_tiles(const sm3_expert_desc* d, bool mx4) {
   const long per_expert = d->rows / (d->num_groups < d->rows ? d->num_groups : d->rows > 0 ? d->rows : 1);
   p.bm = per_expert <= 48 ? 32 : 128;
   p.bn = 128;
-  // Much work per CU: 256 x 256 tiles move half the bytes per product through L2 (16384 rows, 8 experts, 4096 x 1024: 174 -> 149 us,
-  // its input gradient 161 -> 148 us), but a partial last round costs a whole one, so that one runs in quarters in a second
-  // launch.  With one round of a short reduction the second launch costs more than the tile gains (65536 rows, reduction
-  // 1024 to 256 columns: 54 -> 61 us).
+  // Much work per CU: 256 x 256 tiles move half the bytes per product through L2, but a partial last round costs a whole one, so
+  // that one runs in quarters in a second launch.  Measured over 4096 to 65536 rows of 8 uneven experts, 256 to 4096 columns and
+  // reductions of 512 to 4096, bf16, the same operands call after call: where the rule takes them they need 0.77 to 1.02 of the time of
+  // 128 x 128 tiles (16384 rows, 4096 x 1024: 153 -> 136 us, 4096 x 4096: 564 -> 485; 65536 rows, 1024 x 4096: 628 -> 485).  Where it
+  // does not: 1.0 to 1.25 with one to two rounds of 8 or 16 steps (16384 rows, 2048 x 512: 46 -> 51), up to 3.3 with less than
+  // one; a handful of sizes next to its border would have gained up to 14 % (32768 rows, 256 x 4096: 119 -> 103).  (The rounds are
+  // whole ones: a quotient without its rest.)
   const long red_steps = ((mx4 ? (d->red + 127) / 128 * 64 : d->red * 2L) + kStepBytes - 1) / kStepBytes;
   const long some = d->offsets ? (d->num_groups < d->rows ? d->num_groups : d->rows) / 2 : 0;  // half a tile is lost per expert
   const long expected = ((d->rows + 255) / 256 + some) * ((d->cols + 255L) / 256);

@@ -424,8 +424,8 @@ __device__ __forceinline__ v4f mma(v4i q, v4i p, v4f c, int qscale, int pscale, 
 
 // ---- epilogue -----------------------------------------------------------------------------------------------------
 // GELU(h) = h Phi(h) = max(h, 0) - |h| Phi(-|h|), with Phi(-a) = 2^p(a): log2 Phi(-a) is so smooth that a polynomial of degree 7
-// (fitted here by linear programming on [0, 6], minimax in the error relative to |h|) leaves 3.6e-8 |h|, 1.2e-7 |h| with the
-// fp32 rounding of its evaluation; behind 6 |h| Phi(-|h|) is below 6e-9.  One transcendental instruction and 11 others: with the
+// (fitted here by linear programming on [0, 6], minimax in the error relative to |h|, then rounded to fp32) leaves 4.5e-8 |h|,
+// 1.2e-7 |h| with the fp32 rounding of its evaluation; behind 6 |h| Phi(-|h|) is below 6e-9.  One transcendental instruction and 11 others: with the
 // erfc form of Abramowitz & Stegun 7.1.26 (two and 12, error 1e-7) the epilogue of a 4-bit product was bound by GELU.
 // (h / 2 + |h| / 2 is max(h, 0) that lets a NaN through.)
 // Eight at once, step by step, so that no instruction waits for the one before it.
@@ -523,21 +523,24 @@ __device__ __forceinline__ void for_each(F f) { for_each_of(std::make_integer_se
 // ---- the kernel ---------------------------------------------------------------------------------------------------
 // BM output rows (P) x BN output columns (Q); WM x WN waves, MINW waves per SIMD.
 //
-// A workgroup runs through a list of tiles (jobs) as ONE sequence of steps: the loader is two steps ahead of the matrix unit and
-// walks into the next tile while the current one is finished and stored, so a tile costs neither a ramp nor a drain.
-// Two LDS buffers, one barrier per step.  A step is two rounds; while the matrix unit works on one round's fragments, the
+// A workgroup runs through a list of tiles (jobs) as ONE sequence of steps: the loader is NB steps ahead of the matrix unit (two;
+// four in the lone quarters of phase 2) and walks into the next tile while the current one is finished and stored, so a tile costs
+// neither a ramp nor a drain.
+// NB LDS buffers, one barrier per step.  A step is two rounds; while the matrix unit works on one round's fragments, the
 // next round's are read from LDS, piece by piece between the instructions (round 1 reads round 0 of the NEXT step, so the
 // barrier stands between the rounds: by then this step's buffer has been read out and the next one has landed):
 //     round 0: multiply f0 | read f1 from buffer i
-//     wait for the loads of step i + 1 (issued a whole step ago), barrier
+//     wait for the loads of step i + 1 (issued NB - 1 steps ago), barrier
 //     round 1: multiply f1 | read f0 from buffer i + 1 | start loading step i + NB into buffer i
 //
-// Bounds (8 experts, bf16): 16384 x 4096 x 1024 in 149 us = 920 TF/s, the matrix unit 40-60 % busy at the 1.6 GHz the part falls
-// to; 128 x 128 tiles there want 20 TB/s from L2, 256 x 256 ones half of it.  65536 x 1024 x 256 in 55 us: 4 steps per tile,
-// bound by the steps' latency (a lone step takes 0.7-0.9 us whatever its arithmetic).  Storing nothing saved 4 us there;
-// non-temporal stores save 2 us of a lone 4-bit product and cost the feed-forward 3 %, whose second product then finds less of
-// the first one's result in the caches.  MINW: two workgroups of 128 x 128 per CU cover each other's waits; four (32 x 128)
-// where rows are few.
+// Bounds (8 uneven experts, bf16).  16384 x 4096 x 1024: with the same operands call after call 127 us forward, 142 input gradient, 138
+// weight gradient (1080, 970, 1000 TF/s); with other operands each call 149, 156, 166; in a training step, kernel by kernel,
+// 146 + 21 (quarters), 136 + 53, 177.  The matrix unit is 40-60 % busy at the 1.6 GHz the part falls to; 128 x 128 tiles there want
+// 20 TB/s from L2, 256 x 256 ones half of it.  65536 x 1024 x 256: 54, 45, 64 us with the same operands, 78, 59, 85 with others, 80, 61,
+// 61 + 11 (join) in a training step; 4 steps per tile, bound by the steps' latency (a lone step takes 0.7-0.9 us whatever its
+// arithmetic).  Storing nothing saved 4 us there; non-temporal stores save 2 us of a lone 4-bit product and cost the feed-forward
+// 3 %, whose second product then finds less of the first one's result in the caches.  MINW: two workgroups of 128 x 128 per CU
+// cover each other's waits; three of 32 x 128 where rows are few.
 template <int KIND, int MODE, int BM, int BN, int WM, int WN, int MINW, int NB = 2>
 __global__ void __launch_bounds__(WM * WN * 64, MINW) tile_kernel(const Params P) {
   constexpr int WAVES = WM * WN, TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;

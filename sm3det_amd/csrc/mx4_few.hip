@@ -5,7 +5,8 @@
 // its four waves take every fourth step of 128 elements.  A lane loads 16 bytes of a weight row straight into the register
 // operand of the matrix instruction, loads the 32 elements of x that meet them and quantises them in place: the 32 elements of
 // a lane ARE one block, so its maximum needs no other lane.  The waves' fp32 sums are added in LDS in a fixed order.
-// Measured (one token, 4096 x 1024, bf16, GELU): 4.3 us against 1.9 us quantise + 7.6 us tile kernel.
+// Measured (one token, 4096 x 1024, bf16, GELU): 4.3 us against 1.9 us quantise + 7.6 us tile kernel.  With more tiles its time is the
+// rows' quantisation, once per 16 columns (which sizes come here: mx4_gemm.hip).
 #include "expert_plan.h"
 #include "mx4_few.h"
 

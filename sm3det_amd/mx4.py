@@ -200,27 +200,31 @@ class PackedExperts:
 
     def stamp(self, layer):
         """these are `layer`'s parameters as they are now"""
-        self.states = [self._state(p) for p in (layer.w1, layer.b1, layer.w2, layer.b2)]
-
-    @staticmethod
-    def _state(p):
         # (an optimizer that writes by address does not move the version: it counts its steps, MultiTensorAdamW._writer)
-        return p, p.data_ptr(), None if p.is_inference() else p._version, [(w, w.steps) for w in getattr(p, '_sm3_writers', ())]
+        self.states = []
+        for name in ('w1', 'b1', 'w2', 'b2'):
+            p = layer._parameters[name]
+            writers = getattr(p, '_sm3_writers', ())
+            self.states.append((name, p, p.data_ptr(), None if p.is_inference() else p._version, writers, [w.steps for w in writers]))
+        # False: writes may come that the host does not see -- an optimizer step inside a captured graph (capturing it counts as a
+        # step, so this is as old as the rest), parameters that keep no version
+        self.followable = not any(version is None or any(w.captured for w in writers) for *_, version, writers, _ in self.states)
 
     def made_from(self, layer):
         """whether nothing the host sees has changed the parameters since"""
-        return all(p is s[0] and self._state(p)[1:] == s[1:] for p, s in zip((layer.w1, layer.b1, layer.w2, layer.b2), self.states))
-
-    def followable(self):
-        """False: writes may come that the host does not see -- an optimizer step inside a captured graph, parameters that keep no
-        version"""
-        return not any(version is None or any(w.captured for w, _ in writers) for _, _, version, writers in self.states)
+        now = layer._parameters
+        for name, p, address, version, writers, steps in self.states:
+            if now.get(name) is not p or p.data_ptr() != address or (version is not None and p._version != version):
+                return False
+            if getattr(p, '_sm3_writers', ()) != writers or (writers and [w.steps for w in writers] != steps):
+                return False
+        return True
 
     def ffn(self, xslot, offsets):
         return expert_ffn(xslot, self.w1, self.b1, self.w2, self.b2, offsets)
 
     def __getstate__(self):  # (a copy of the layer has parameters of its own: MoE_layer.__setstate__ stamps)
-        return {k: v for k, v in self.__dict__.items() if k != 'states'}
+        return {k: v for k, v in self.__dict__.items() if k not in ('states', 'followable')}
 
 
 def quantize_experts(module):

@@ -26,8 +26,19 @@ struct Plan {
 // elements of an operand's row (16 bits), and between rows: byte offsets inside a tile of up to 256 rows have 31 bits
 constexpr long kMostElements = 1L << 22;
 
+// A grid's first dimension holds fewer than 2^32 threads; a launch of more ends without an error and without its work.
+inline bool launchable(long blocks, long threads) { return blocks * threads < 1L << 32; }
+
+// workgroups per XCD: as many as are resident at once, each with its share of the jobs -- at most kMaxJobs of them
+inline long workgroups(const Plan& pl, int per_cu) {
+  const long most = (long)kNumCU / kNumXCD * per_cu, least = (pl.per_xcd + kMaxJobs - 1) / kMaxJobs;
+  return pl.per_xcd < most ? pl.per_xcd : most > least ? most : least;
+}
+
 // jobs are counted in 31 bits
-inline bool fits(const Plan& p) { return (double)p.per_xcd * kNumXCD < 2.0e9 && (double)p.units < 2.0e9; }
+inline bool fits(const Plan& p) {
+  return (double)p.per_xcd * kNumXCD < 2.0e9 && (double)p.units < 2.0e9 && launchable(workgroups(p, 3) * kNumXCD, p.coarse ? 512 : 256);
+}
 
 inline int check_desc(const sm3_expert_desc* d, bool mx4) {
   if (!d || d->num_groups < 1 || d->rows < 0 || d->rows > 0x7fffff00L || d->red < 1 || d->cols < 1) return SM3_ERR_INVALID_ARG;
@@ -306,12 +317,7 @@ inline Params params_of(const sm3_expert_desc* d, const Plan& pl, bool mx4, cons
   return P;
 }
 
-// as many workgroups as are resident at once (a multiple of the XCDs), each with its share of the jobs -- at most kMaxJobs of them
-inline dim3 grid_of(const Plan& pl, int per_cu) {
-  const long most = (long)kNumCU / kNumXCD * per_cu, least = (pl.per_xcd + kMaxJobs - 1) / kMaxJobs;
-  const long each = pl.per_xcd < most ? pl.per_xcd : most > least ? most : least;
-  return dim3((unsigned)(each * kNumXCD));
-}
+inline dim3 grid_of(const Plan& pl, int per_cu) { return dim3((unsigned)(workgroups(pl, per_cu) * kNumXCD)); }
 
 inline int finish(const Params& P, const Plan& pl, const sm3_expert_desc* d, hipStream_t st) {
   if (d->mode == SM3_GEMM_TN) {

@@ -16,7 +16,8 @@ namespace {
 // 1024 (33 M) 102 / 188 against 30 / 31.
 bool few(const sm3_expert_desc* d) {
   const long experts = d->num_groups < d->rows ? d->num_groups : d->rows;
-  if (d->p_scales || d->rows > 16 * experts || row_tiles(d->rows, d->num_groups, d->offsets != nullptr, 16) >= 65536) return false;
+  if (d->p_scales || d->rows > 16 * experts) return false;
+  if (row_tiles(d->rows, d->num_groups, d->offsets != nullptr, 16) >= 65536 || !launchable((d->cols + 15) / 16, 256)) return false;
   const double work = (double)(d->rows / 16 + experts) * ((d->cols + 15) / 16) * ((d->red + 127) / 128 * 128);
   return d->rows <= 16 || work <= (d->type == SM3_DT_F32 ? 2.5e6 : 3.4e6);
 }

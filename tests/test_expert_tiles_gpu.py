@@ -150,3 +150,23 @@ def test_a_bias_row_of_2_to_the_32_bytes(bias):
     del w, b, y
     torch.cuda.empty_cache()
     assert rest == 2 * (n - 900)
+
+
+@pytest.mark.parametrize('n', ((1 << 28) - 16, 1 << 28, (1 << 28) + 40))
+def test_few_rows_of_very_many_columns(n):
+    """a launch holds fewer than 2^32 threads: behind 2^28 columns the one-launch kernel of few rows would need more"""
+    from sm3det_amd import mx4
+    codes = torch.zeros(n, 64, dtype=torch.uint8, device='cuda')
+    scales = torch.full((n, 4), 127, dtype=torch.uint8, device='cuda')
+    some = torch.cat([torch.arange(200), n // 2 + torch.arange(200), n - 200 + torch.arange(200)]).cuda()
+    codes[some] = torch.randint(0, 256, (600, 64), generator=torch.Generator(device='cuda').manual_seed(1), device='cuda').to(torch.uint8)
+    w = mx4.Mx4Tensor(codes, scales, 128)
+    x = _randn(2, 3, 128, dtype=torch.bfloat16)
+    y = mx4.linear(x, w)
+    X, W = _values(mx4.quantize(x)), _values(mx4.Mx4Tensor(codes[some], scales[some], 128))
+    ref = X @ W.t()
+    assert_within(y[:, some], ref, bound(ref, X.abs() @ W.abs().t(), 128, torch.bfloat16))
+    rest = int(y.count_nonzero()) - int(y[:, some].count_nonzero())
+    del w, codes, scales, y
+    torch.cuda.empty_cache()
+    assert rest == 0

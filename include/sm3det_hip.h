@@ -663,7 +663,8 @@ int sm3_gfl_loss_bwd(const float* cls, const float* bbox, const float* anchors, 
  * and sign).  k elements are padded with zeros to kp = k rounded up to a multiple of 128.  codes (rows, kp / 2): element 2 i in
  * the low, 2 i + 1 in the high nibble of byte i; scales (rows, kp / 32).
  * quantize: byte = max(floor(log2 max|x|) - 2 + 127, 0); elements round to nearest, ties to the even code, beyond 6 to 6; a block
- * that holds an infinity or a NaN gets byte 255 (the whole block is NaN).  x: `rows` rows of k elements, ld elements apart.
+ * that holds an infinity or a NaN gets byte 255 (the whole block is NaN).  x: `rows` rows of k elements (at most 2^31 - 128), ld
+ * elements apart.
  * dequantize: y (rows, k) contiguous, rounded to nearest even. */
 int sm3_mx4_quantize(const void* x, int type, long rows, int k, long ld, uint8_t* codes, uint8_t* scales,
                      sm3_stream_t stream);
@@ -675,6 +676,7 @@ int sm3_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, long rows, i
  *   mode SM3_GEMM_NN: out (rows, cols) = p (rows, red) . q[g] (red, cols)
  *   mode SM3_GEMM_TN: out[g] (rows_out, cols) = p (rows of g, rows_out)^T . q (rows of g, cols); bias_grad[g] (rows_out) = column
  *                     sums of p over the rows of g (may be NULL).  Experts without rows get zeros.
+ * Rows of p and q hold at most 2^22 elements, cols is at most 2^30, num_groups at most 65535 (else SM3_ERR_UNSUPPORTED).
  * 16-bit: p, q of type `type` (F16 | BF16), ldp / ldq elements between rows (>= the row's length); NT / NN weights of expert g
  * start at q + g * cols * ldq (NN: g * red * ldq).  Rows that do not start at 16-byte addresses or are no multiple of 8 long are
  * copied into padded ones in the workspace first.  out contiguous, out_type = type.

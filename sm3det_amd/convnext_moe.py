@@ -149,10 +149,13 @@ class MoE_layer(nn.Module):
         if not packed.followable:
             from . import mx4
             packed = mx4.PackedExperts(self)
-        elif packed.b1.is_cuda and torch.cuda.is_current_stream_capturing():
-            held = self.__dict__.setdefault('_mx4_captured', [])  # the graph reads them in every replay
-            if not any(h is packed for h in held):
-                held.append(packed)
+        elif packed.b1.is_cuda:
+            if torch.cuda.is_current_stream_capturing():
+                held = self.__dict__.setdefault('_mx4_captured', [])  # the graph reads them in every replay
+                if not any(h is packed for h in held):
+                    held.append(packed)
+            else:
+                packed.read_here()
         return packed.ffn
 
     def __getstate__(self):  # copies and pickles: a snapshot that is of use goes along, what graphs of this layer read does not

@@ -199,7 +199,8 @@ class PackedExperts:
         self.stamp(layer)
 
     def stamp(self, layer):
-        """these are `layer`'s parameters as they are now"""
+        """these are `layer`'s parameters as they are now, packed (or copied) on the current stream"""
+        self.stream = torch._C._cuda_getCurrentRawStream(self.b1.device.index) if self.b1.is_cuda else None
         # (an optimizer that writes by address does not move the version: it counts its steps, MultiTensorAdamW._writer)
         self.states = []
         for name in ('w1', 'b1', 'w2', 'b2'):
@@ -220,11 +221,19 @@ class PackedExperts:
                 return False
         return True
 
+    def read_here(self):
+        """the current stream is about to read them: dropped before it has, they stay allocated until then"""
+        device = self.b1.device
+        if torch._C._cuda_getCurrentRawStream(device.index) != self.stream:
+            stream = torch.cuda.current_stream(device)
+            for t in (self.w1.codes, self.w1.scales, self.b1, self.w2.codes, self.w2.scales, self.b2):
+                t.record_stream(stream)
+
     def ffn(self, xslot, offsets):
         return expert_ffn(xslot, self.w1, self.b1, self.w2, self.b2, offsets)
 
     def __getstate__(self):  # (a copy of the layer has parameters of its own: MoE_layer.__setstate__ stamps)
-        return {k: v for k, v in self.__dict__.items() if k not in ('states', 'followable')}
+        return {k: v for k, v in self.__dict__.items() if k not in ('states', 'followable', 'stream')}
 
 
 def quantize_experts(module):

@@ -183,3 +183,26 @@ def test_a_captured_forward_keeps_the_snapshot_it_was_captured_with(net):
         torch.cuda.synchronize()
         del junk
         assert _same(out, want)
+
+
+def test_a_forward_on_another_stream_outlives_what_it_reads(net):
+    """the packed experts are dropped and their memory is used again while a side stream has yet to run the forward"""
+    from sm3det_amd import mx4
+    mx4.quantize_experts(net)
+    want = [o.clone() for o in _out(net)]
+    sizes = [t.numel() for m in _layers(net) for t in (m._mx4.w1.codes, m._mx4.w1.scales, m._mx4.w2.codes, m._mx4.w2.scales)]
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        _out(net)  # (allocations of the side stream, first launches)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(1_000_000_000)
+        out = _out(net)
+    net.train().eval()
+    junk = [torch.full((n,), 0x11, dtype=torch.uint8, device='cuda') for n in sizes * 3]
+    torch.cuda.current_stream().synchronize()
+    assert not s.query()  # (the side stream still sleeps: what was written above, it finds)
+    s.synchronize()
+    del junk
+    same = _same(out, want)
+    assert same

@@ -26,8 +26,9 @@ DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
 def has_tangent(*tensors):
-    """whether forward-mode differentiation (which no_grad() does not end) would have to follow one of the tensors"""
-    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    """whether forward-mode differentiation (which no_grad() does not end) would have to follow one of the tensors; asked where
+    `forward_ad._current_level` says that it is on"""
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def check_offsets(offsets, num_groups, device, name):
@@ -173,7 +174,7 @@ def expert_linear(x, w, offsets, b=None):
             raise SM3Error(f'expert_linear: b must be {tuple(w.shape[:2])} of {x.dtype} or float32, got {tuple(b.shape)} of '
                            f'{b.dtype}')
         b = b.contiguous()
-    if has_tangent(x, w, b):
+    if forward_ad._current_level >= 0 and has_tangent(x, w, b):
         raise SM3Error('expert_linear: an input carries a forward-mode tangent; only backward-mode derivatives are implemented')
     offsets = check_offsets(offsets, w.shape[0], x.device, 'expert_linear')
     # (copies are made here, where autograd sees them: what it saves are then the caller's tensors or lead to them)

@@ -13,6 +13,7 @@ dequantised.  Inference only: a call that autograd would have to differentiate i
 experts of a backbone's MoE blocks (mmrotate/models/backbones/convnext_moe.py:226-248) on these products in evaluation.
 """
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib_backbone as LB
 from ._lib import SM3Error, check, lib, require_gpu
@@ -97,7 +98,7 @@ def _call(name, device, nbytes, *args):
 def _no_grad(what, *tensors):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise SM3Error(f'{what} is for inference: an input requires a gradient (use torch.no_grad())')
-    if has_tangent(*tensors):
+    if forward_ad._current_level >= 0 and has_tangent(*tensors):
         raise SM3Error(f'{what} is for inference: an input carries a forward-mode tangent')
 
 
